@@ -1,0 +1,240 @@
+// Global gradient norm over many tensors, and clipping by it.
+//
+//   total = sqrt(sum over all tensors and elements of g^2)
+//   g     = g * min(1, max_norm / (total + eps))
+//
+// One launch covers up to PER tensors: their addresses and sizes travel in the kernel's arguments
+// (nothing is copied to the device, and a captured graph holds them by value).  The squares are
+// summed in 64 bits: an fp32 square leaves its range for |g| above 1.8e19 or below 1e-22, and the
+// sum runs over up to 1e10 elements.  Partial sums are written per workgroup and joined in a fixed
+// order: no atomics, the same bits every time.
+#include <math.h>
+
+#include "common.h"
+
+namespace {
+constexpr int NT = 256;
+constexpr int PER = 128;            // tensors per launch (kernel arguments stay under 4 KiB)
+constexpr int CHUNK = 16384;        // elements a workgroup takes at a time
+constexpr int NORM_GRID = 2048, CLIP_GRID = 4096;
+
+struct Tensors {
+  const void* src[PER];
+  void* dst[PER];
+  int64_t n[PER];                   // elements | type << 60
+  int first[PER + 1];               // chunks before tensor i
+  int count;
+};
+
+__device__ __forceinline__ int owner(const Tensors& t, int chunk) {
+  int lo = 0, hi = t.count;         // first[lo] <= chunk < first[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (t.first[mid] <= chunk) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// 16-byte vectors with the element's alignment: a gradient that is a view into a flat buffer may
+// start anywhere
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  typedef T type __attribute__((ext_vector_type(N)));
+  typedef type at __attribute__((aligned(sizeof(T))));
+};
+
+template <typename T>
+__device__ __forceinline__ double sum_squares(const T* p, int len) {
+  constexpr int N = Vec<T>::N, STEP = NT * N;
+  double s = 0.0;
+  int i = threadIdx.x * N;
+  for (; i + 3 * STEP + N <= len; i += 4 * STEP) {
+    typename Vec<T>::type v[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) v[u] = *(const typename Vec<T>::at*)(p + i + u * STEP);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int k = 0; k < N; ++k) {
+        const double d = (double)(float)v[u][k];
+        s = fma(d, d, s);
+      }
+  }
+  for (; i < len; i += STEP)
+    for (int k = 0; k < N && i + k < len; ++k) {
+      const double d = (double)(float)p[i + k];
+      s = fma(d, d, s);
+    }
+  return s;
+}
+
+__device__ __forceinline__ double block_sum_f64(double v, double* red) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double s = 0.0;
+  for (int i = 0; i < (int)(blockDim.x >> 6); ++i) s += red[i];
+  return s;
+}
+
+__global__ __launch_bounds__(NT) void grads_norm_kernel(Tensors t, double* __restrict__ part) {
+  __shared__ double red[NT / 64];
+  double s = 0.0;
+  for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
+    const int i = owner(t, c);
+    const int64_t n = t.n[i] & ((1ll << 60) - 1), at = (int64_t)(c - t.first[i]) * CHUNK;
+    const int len = (int)(n - at < CHUNK ? n - at : CHUNK), type = (int)(t.n[i] >> 60);
+    if (type == 0) s += sum_squares((const float*)t.src[i] + at, len);
+    else if (type == 1) s += sum_squares((const bf16*)t.src[i] + at, len);
+    else s += sum_squares((const _Float16*)t.src[i] + at, len);
+  }
+  s = block_sum_f64(s, red);
+  if (threadIdx.x == 0) part[blockIdx.x] = s;
+}
+
+__global__ __launch_bounds__(1024) void grads_norm_join_kernel(const double* __restrict__ part, int P,
+                                                               double* __restrict__ sumsq) {
+  __shared__ double red[16];
+  double s = 0.0;
+  for (int i = threadIdx.x; i < P; i += 1024) s += part[i];
+  s = block_sum_f64(s, red);
+  if (threadIdx.x == 0) sumsq[0] = s;
+}
+
+template <typename TS, typename TD>
+__device__ __forceinline__ void scaled(const TS* src, TD* dst, int len, float f) {
+  constexpr int N = Vec<TS>::N;
+  typedef TD dvec __attribute__((ext_vector_type(N)));
+  typedef dvec dat __attribute__((aligned(sizeof(TD))));
+  for (int i = threadIdx.x * N; i < len; i += NT * N) {
+    if (i + N <= len) {
+      const typename Vec<TS>::type v = *(const typename Vec<TS>::at*)(src + i);
+      dvec o;
+#pragma unroll
+      for (int k = 0; k < N; ++k) o[k] = (TD)((float)v[k] * f);
+      *(dat*)(dst + i) = o;
+    } else {
+      for (int k = i; k < len; ++k) dst[k] = (TD)((float)src[k] * f);
+    }
+  }
+}
+
+__device__ __forceinline__ float coefficient(float norm, float max_norm, float eps) {
+  const float c = max_norm / (norm + eps);
+  return c > 1.f ? 1.f : c;         // a NaN norm stays NaN
+}
+
+// dst = src * coefficient; norm_out gets the norm once.  In place with a coefficient of 1 nothing
+// changes, so nothing is read.
+__global__ __launch_bounds__(NT) void grads_clip_kernel(Tensors t, int dtype,
+                                                        const double* __restrict__ sumsq,
+                                                        float max_norm, float eps,
+                                                        float* __restrict__ norm_out) {
+  const float norm = (float)sqrt(sumsq[0]);
+  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = norm;
+  const float f = coefficient(norm, max_norm, eps);
+  if (dtype < 0 && f == 1.f) return;
+  for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
+    const int i = owner(t, c);
+    const int64_t n = t.n[i] & ((1ll << 60) - 1), at = (int64_t)(c - t.first[i]) * CHUNK;
+    const int len = (int)(n - at < CHUNK ? n - at : CHUNK), type = (int)(t.n[i] >> 60);
+    const int to = dtype < 0 ? type : dtype;
+    auto run = [&](auto* src) {
+      if (to == 0) scaled(src + at, (float*)t.dst[i] + at, len, f);
+      else if (to == 1) scaled(src + at, (bf16*)t.dst[i] + at, len, f);
+      else scaled(src + at, (_Float16*)t.dst[i] + at, len, f);
+    };
+    if (type == 0) run((const float*)t.src[i]);
+    else if (type == 1) run((const bf16*)t.src[i]);
+    else run((const _Float16*)t.src[i]);
+  }
+}
+
+// calls f(Tensors) for each launch's share of the list; false if an entry cannot be served
+template <typename F>
+bool for_each_launch(const void* const* src, void* const* dst, const int64_t* n, const int32_t* type,
+                     int64_t count, F f) {
+  Tensors t;
+  t.count = 0;
+  t.first[0] = 0;
+  for (int64_t i = 0; i < count; ++i) {
+    if (n[i] < 0 || type[i] < 0 || type[i] > 2 || (n[i] > 0 && (!src[i] || (dst && !dst[i])))) return false;
+    if (n[i] == 0) continue;
+    const int64_t chunks = (n[i] + CHUNK - 1) / CHUNK;
+    if (chunks > (1 << 30)) return false;
+    if (t.count == PER || t.first[t.count] + chunks > (1 << 30)) {
+      f(t);
+      t.count = 0;
+    }
+    t.src[t.count] = src[i];
+    t.dst[t.count] = dst ? dst[i] : nullptr;
+    t.n[t.count] = n[i] | ((int64_t)type[i] << 60);
+    t.first[t.count + 1] = t.first[t.count] + (int)chunks;
+    ++t.count;
+  }
+  if (t.count) f(t);
+  return true;
+}
+int grid_of(const Tensors& t, int most) {
+  const int c = t.first[t.count];
+  return c < most ? c : most;
+}
+}  // namespace
+
+extern "C" int64_t prfl_grads_parts(const int64_t* n, int64_t count) {
+  int64_t chunks = 0, live = 0;
+  for (int64_t i = 0; i < count; ++i)
+    if (n[i] > 0) chunks += (n[i] + CHUNK - 1) / CHUNK, ++live;
+  const int64_t most = ((live + PER - 1) / PER + chunks / (1 << 30)) * NORM_GRID;
+  return chunks < most ? chunks : most;
+}
+
+extern "C" int prfl_grads_sumsq(const void* const* grads, const int64_t* n, const int32_t* type,
+                                int64_t count, double* part, int64_t parts, double* sumsq,
+                                void* stream) {
+  if (count < 0 || !sumsq || (count && (!grads || !n || !type)) || parts < prfl_grads_parts(n, count))
+    return (int)hipErrorInvalidValue;
+  hipStream_t s = (hipStream_t)stream;
+  int P = 0;
+  if (!for_each_launch(grads, nullptr, n, type, count, [](const Tensors&) {}))
+    return (int)hipErrorInvalidValue;
+  for_each_launch(grads, nullptr, n, type, count, [&](const Tensors& t) {
+    const int g = grid_of(t, NORM_GRID);
+    hipLaunchKernelGGL(grads_norm_kernel, dim3(g), dim3(NT), 0, s, t, part + P);
+    P += g;
+  });
+  hipLaunchKernelGGL(grads_norm_join_kernel, dim3(1), dim3(1024), 0, s, part, P, sumsq);
+  PRFL_LAUNCH_CHECK();
+  return 0;
+}
+
+extern "C" int prfl_grads_clip(const void* const* grads, void* const* out, const int64_t* n,
+                               const int32_t* type, int64_t count, int out_type, const double* sumsq,
+                               float max_norm, float eps, float* norm, void* stream) {
+  if (count < 0 || !sumsq || out_type > 2 || (count && (!grads || !n || !type)) || (out_type >= 0 && !out) ||
+      !(max_norm >= 0.f) || !(eps >= 0.f))
+    return (int)hipErrorInvalidValue;
+  hipStream_t s = (hipStream_t)stream;
+  void* const* dst = out ? out : (void* const*)grads;
+  if (!for_each_launch(grads, dst, n, type, count, [](const Tensors&) {}))
+    return (int)hipErrorInvalidValue;
+  bool first = true;
+  auto launch = [&](const Tensors& t) {
+    const int g = grid_of(t, CLIP_GRID);
+    hipLaunchKernelGGL(grads_clip_kernel, dim3(g < 1 ? 1 : g), dim3(NT), 0, s, t, out ? out_type : -1,
+                       sumsq, max_norm, eps, first ? norm : nullptr);
+    first = false;
+  };
+  for_each_launch(grads, dst, n, type, count, launch);
+  if (first && norm) {
+    Tensors none;
+    none.count = 0;
+    none.first[0] = 0;
+    launch(none);
+  }
+  PRFL_LAUNCH_CHECK();
+  return 0;
+}

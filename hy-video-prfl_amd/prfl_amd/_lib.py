@@ -78,13 +78,23 @@ SIGNATURES = {
                             P],
     "prfl_query_pool_bwd": [P, P, I64, P, I64, I64, P, P, I64, I64, I64, I64, F32, P, I64, P, I64,
                             I64, P, I64, P],
+    "prfl_layer_norm_fwd": [P, I32, I64, I64, I64, P, P, I32, F32, P, I32, I64, P, P, P],
+    "prfl_layer_norm_bwd": [P, I32, I64, P, I32, I64, P, P, I64, I64, P, I32, P, I64, P, P, P, P],
+    "prfl_layer_norm_parts": [I64, I64, I32],
+    "prfl_grads_parts": [P, I64],
+    "prfl_grads_sumsq": [P, P, P, I64, P, I64, P, P],
+    "prfl_grads_clip": [P, P, P, P, I64, I32, P, F32, F32, P, P],
+    "prfl_quant_mxfp4": [P, I32, I64, I64, I64, P, P, P],
+    "prfl_dequant_mxfp4": [P, P, I64, I64, P, I32, I64, P],
+    "prfl_gemm_mxfp4": [P, P, P, P, P, P, I64, I64, I64, I64, P],
     "prfl_prof_enable": [I32],
     "prfl_prof_collect": [P, P, P, I32],
     "prfl_prof_clock": [P, P, P, P],
 }
 
 # entries that return a value other than a hipError_t code
-RESTYPES = {"prfl_attn_fwd_ws_bytes": I64, "prfl_attn_vt_bytes": I64, "prfl_attn_fwd_fp8_ws_bytes": I64, "prfl_attn_bwd_ws_bytes": I64}
+RESTYPES = {"prfl_attn_fwd_ws_bytes": I64, "prfl_attn_vt_bytes": I64, "prfl_attn_fwd_fp8_ws_bytes": I64, "prfl_attn_bwd_ws_bytes": I64,
+            "prfl_layer_norm_parts": I64, "prfl_grads_parts": I64}
 
 # kernel ids of the profiling hooks (csrc/common.h)
 KID = dict(gemm=0, attn_fwd=1, attn_fwd_short=2, attn_bwd_dkdv=3, attn_bwd_dq=4, ln=5, rms=6,
@@ -114,6 +124,14 @@ def call(name, *args):
     if rc != 0:
         raise RuntimeError(f"{name} failed with hipError {rc}")
     return rc
+
+
+def call_on(device, name, *args):
+    """call(name, *args, stream) on `device`'s current stream, whichever device is current."""
+    if torch.cuda.current_device() == device.index:
+        return call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+    with torch.cuda.device(device):
+        return call(name, *args, torch.cuda.current_stream(device).cuda_stream)
 
 
 def stream_ptr(device=None):

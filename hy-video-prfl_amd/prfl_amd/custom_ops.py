@@ -12,6 +12,10 @@ whose CUDA (= HIP) implementations call the C ABI of ``libprfl_hip.so`` (include
 | prfl::query_pool (+ _backward)   | the 1-query `nn.MultiheadAttention` core (`network.py:80`)  |
 | prfl::unipc_step (+ _backward)   | `FlowUniPCMultistepScheduler.step`'s element-wise body      |
 |                                  | (`fm_solvers_unipc.py:350-626`)                              |
+| prfl::layer_norm (+ _backward)   | `nn.LayerNorm` over the last axis, trained (`model.py:304`, |
+|                                  | `:360-372`): any width to 16384, fp32 / bf16 / fp16         |
+| prfl::linear_mxfp4 (+ _backward) | a frozen trunk's `nn.Linear` with its weight in microscaled |
+|                                  | fp4 (no counterpart in the bf16-only reference)             |
 
 Because these are dispatcher ops, autograd sees ordinary nodes: `torch.utils.checkpoint`
 (non-reentrant, as `apply_fsdp_checkpointing` installs it) recomputes them, FSDP's
@@ -425,3 +429,116 @@ def unipc_update(model_output, sample, last_sample, hist1, hist2, coef, corr_ord
     m_t, sample_c, prev = unipc_step(model_output, sample, last_sample, hist1, hist2,
                                      [float(c) for c in coef], int(corr_order), int(pred_order))
     return m_t, (sample_c if corr_order else sample), prev
+
+
+# ================================================================ layer norm (last axis) ====
+@torch.library.custom_op("prfl::layer_norm", mutates_args=(), device_types="cuda")
+def _layer_norm(x: Tensor, w: Optional[Tensor], b: Optional[Tensor], eps: float,
+                out_dtype: Optional[torch.dtype]) -> Tuple[Tensor, Tensor, Tensor]:
+    """(y in out_dtype or x's, mean, rstd fp32 of x's leading shape)."""
+    return ops.layer_norm_fwd(x, w, b, eps, out_dtype)
+
+
+@_layer_norm.register_fake
+def _(x, w, b, eps, out_dtype):
+    return (x.new_empty(x.shape, dtype=out_dtype or x.dtype), x.new_empty(x.shape[:-1], dtype=F32),
+            x.new_empty(x.shape[:-1], dtype=F32))
+
+
+@torch.library.custom_op("prfl::layer_norm_backward", mutates_args=(), device_types="cuda")
+def layer_norm_backward(dy: Tensor, x: Tensor, mean: Tensor, rstd: Tensor, w: Optional[Tensor],
+                        need_dx: bool, need_dw: bool, need_db: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    """(dx in x's type, dw, db fp32 [C]), empty where not needed."""
+    dx, dw, db = ops.layer_norm_bwd(dy, x, mean, rstd, w, need_dx, need_dw, need_db)
+    return (_empty(x) if dx is None else dx, _empty(x, F32) if dw is None else dw,
+            _empty(x, F32) if db is None else db)
+
+
+@layer_norm_backward.register_fake
+def _(dy, x, mean, rstd, w, need_dx, need_dw, need_db):
+    C = x.shape[-1]
+    return (x.new_empty(x.shape) if need_dx else _empty(x),
+            x.new_empty((C,), dtype=F32) if need_dw else _empty(x, F32),
+            x.new_empty((C,), dtype=F32) if need_db else _empty(x, F32))
+
+
+def _ln_setup(ctx, inputs, output):
+    x, w, b, eps, out_dtype = inputs
+    _, mean, rstd = output
+    ctx.mark_non_differentiable(mean, rstd)
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(x, w, mean, rstd)
+    ctx.b_dtype = b.dtype if b is not None else None
+
+
+def _ln_bwd(ctx, dy, _dmean, _drstd):
+    x, w, mean, rstd = ctx.saved_tensors
+    rx, rw, rb = ctx.needs_input_grad[:3]
+    if dy is None:
+        return (None,) * 5
+    dx, dw, db = layer_norm_backward(dy, x, mean, rstd, w, rx, rw, rb)
+    return (dx if rx else None, dw.to(w.dtype) if rw else None, db.to(ctx.b_dtype) if rb else None,
+            None, None)
+
+
+_layer_norm.register_autograd(_ln_bwd, setup_context=_ln_setup)
+
+
+def layer_norm(x, w=None, b=None, eps=1e-5, out_dtype=None):
+    """Layer norm over the last axis of x with optional weight and bias, differentiable in all
+    three; the gradients come in their own types, summed over the rows in fp32."""
+    return _layer_norm(x, w, b, float(eps), out_dtype)[0]
+
+
+# ===================================================== Linear with a frozen fp4 weight ======
+@torch.library.custom_op("prfl::linear_mxfp4", mutates_args=(), device_types="cuda")
+def linear_mxfp4(x: Tensor, wq: Tensor, ws: Tensor, out_features: int,
+                 bias: Optional[Tensor]) -> Tensor:
+    """y [..., N] bf16 = x W^T + bias with W [N, K] as ops.quant_mxfp4 keeps it and x [..., K]
+    quantised in the call.  Differentiable in x (its quantisation taken as the identity) and bias."""
+    return ops.linear_mxfp4(x, wq, ws, out_features, bias)
+
+
+@linear_mxfp4.register_fake
+def _(x, wq, ws, out_features, bias):
+    return x.new_empty((*x.shape[:-1], out_features), dtype=BF16)
+
+
+@torch.library.custom_op("prfl::linear_mxfp4_backward", mutates_args=(), device_types="cuda")
+def linear_mxfp4_backward(dy: Tensor, wq: Tensor, ws: Tensor, in_features: int, need_dx: bool,
+                          need_db: bool) -> Tuple[Tensor, Tensor]:
+    """(dx [..., K] bf16 = dy W, db fp32 [N] = colsum(dy)), empty where not needed."""
+    dx = ops.linear_mxfp4_dx(dy, wq, ws, in_features) if need_dx else _empty(dy, BF16)
+    db = _empty(dy, F32)
+    if need_db:
+        N = dy.shape[-1]
+        d = dy.reshape(-1, N).to(BF16)
+        if N % 8:
+            d = torch.nn.functional.pad(d, (0, -N % 8))
+        db = ops.colsum(d.contiguous())[:N].contiguous()
+    return dx, db
+
+
+@linear_mxfp4_backward.register_fake
+def _(dy, wq, ws, in_features, need_dx, need_db):
+    return (dy.new_empty((*dy.shape[:-1], in_features), dtype=BF16) if need_dx else _empty(dy, BF16),
+            dy.new_empty((dy.shape[-1],), dtype=F32) if need_db else _empty(dy, F32))
+
+
+def _mx_setup(ctx, inputs, output):
+    x, wq, ws, out_features, bias = inputs
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(wq, ws)
+    ctx.K, ctx.x_dtype = x.shape[-1], x.dtype
+
+
+def _mx_bwd(ctx, dy):
+    wq, ws = ctx.saved_tensors
+    rx, rb = ctx.needs_input_grad[0], ctx.needs_input_grad[4]
+    if dy is None:
+        return (None,) * 5
+    dx, db = linear_mxfp4_backward(dy, wq, ws, ctx.K, rx, rb)
+    return dx.to(ctx.x_dtype) if rx else None, None, None, None, db.to(BF16) if rb else None
+
+
+linear_mxfp4.register_autograd(_mx_bwd, setup_context=_mx_setup)

@@ -3,6 +3,7 @@
 All tensors are 2-D row-major views ``[rows, cols]`` with unit column stride; row strides are
 passed through, so q/k/v slices of the fused QKV output need no copy.
 """
+import ctypes
 import math
 
 import torch
@@ -412,6 +413,268 @@ def rope_table(freqs_complex, device):
     """complex freqs [1024, 64] (model.py:521-526) -> fp32 (cos, sin) table on device."""
     t = torch.view_as_real(freqs_complex.to(torch.complex128)).to(torch.float32).contiguous()
     return t.to(device)
+
+
+# ---------------------------------------------------------------- layer norm (csrc/layernorm.hip)
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _type(t, what):
+    if t not in TYPES:
+        raise ValueError(f"{what}: fp32, bf16 or fp16, got {t}")
+    return TYPES[t]
+
+
+def _one_device(what, *tensors):
+    _lib.require_gpu(*tensors)
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+    return dev
+
+
+def _rows(t, C):
+    """[..., C] as [rows, C] with unit column stride (a view where the strides allow it)."""
+    t = t.reshape(-1, C) if t.dim() != 2 else t
+    return t if t.stride(1) == 1 or C == 1 else t.contiguous()
+
+
+def layer_norm_fwd(x, w=None, b=None, eps=1e-5, out_dtype=None):
+    """LN over the last axis of x [..., C] (C <= 16384), times w plus b ([C] each, or None):
+    returns (y in out_dtype or x's, mean, rstd fp32 of x's leading shape)."""
+    C = x.shape[-1] if x.dim() else 0
+    if not 1 <= C <= 16384:
+        raise ValueError(f"layer_norm: a last axis of 1 to 16384, got {tuple(x.shape)}")
+    dev = _one_device("layer_norm", x, w, b)
+    ydt = x.dtype if out_dtype is None else out_dtype
+    xt, yt, wt = _type(x.dtype, "layer_norm x"), _type(ydt, "layer_norm out_dtype"), 0
+    for v in (w, b):
+        if v is not None:
+            wt = _type(v.dtype, "layer_norm w")
+            if v.shape != (C,) or (w is not None and v.dtype != w.dtype):
+                raise ValueError(f"layer_norm: w and b are [{C}] of one type")
+    if not eps >= 0:
+        raise ValueError(f"layer_norm: eps is not negative, got {eps}")
+    w, b = (v if v is None else v.contiguous() for v in (w, b))
+    x2 = _rows(x, C)
+    L = x2.shape[0]
+    y = torch.empty(x.shape, dtype=ydt, device=dev)
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    _lib.call_on(dev, "prfl_layer_norm_fwd", x2.data_ptr(), xt, x2.stride(0), L, C, _addr(w),
+                 _addr(b), wt, eps, y.data_ptr(), yt, C, mean.data_ptr(), rstd.data_ptr())
+    return y, mean, rstd
+
+
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
+def layer_norm_bwd(dy, x, mean, rstd, w=None, want_dx=True, want_dw=None, want_db=True):
+    """Backward of layer_norm_fwd: (dx in x's type, dw, db fp32 [C]; None where not wanted).  dy has
+    the forward's output type; dw is given by default where w is."""
+    C = x.shape[-1]
+    dev = _one_device("layer_norm", x, dy, mean, rstd, w)
+    if dy.shape != x.shape or mean.numel() * C != x.numel() or rstd.numel() != mean.numel():
+        raise ValueError("layer_norm: dy has x's shape, mean and rstd one value a row")
+    if mean.dtype != torch.float32 or rstd.dtype != torch.float32:
+        raise ValueError("layer_norm: mean and rstd are the forward's fp32")
+    if w is not None and w.shape != (C,):
+        raise ValueError(f"layer_norm: w is [{C}]")
+    xt, yt = _type(x.dtype, "layer_norm x"), _type(dy.dtype, "layer_norm dy")
+    wt = 0 if w is None else _type(w.dtype, "layer_norm w")
+    want_dw = w is not None if want_dw is None else want_dw
+    x2, dy2 = _rows(x, C), _rows(dy, C)
+    L = x2.shape[0]
+    mean, rstd = mean.contiguous(), rstd.contiguous()
+    w = None if w is None else w.contiguous()
+    f32 = dict(dtype=torch.float32, device=dev)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
+    dw = torch.empty(C, **f32) if want_dw else None
+    db = torch.empty(C, **f32) if want_db else None
+    part = None
+    if want_dw or want_db:
+        n = _lib.load().prfl_layer_norm_parts(L, C, xt)
+        part = torch.empty(max(1, n * C * (int(want_dw) + int(want_db))), **f32)
+    _lib.call_on(dev, "prfl_layer_norm_bwd", dy2.data_ptr(), yt, dy2.stride(0), x2.data_ptr(), xt,
+                 x2.stride(0), mean.data_ptr(), rstd.data_ptr(), L, C, _addr(w), wt, _addr(dx), C,
+                 _addr(dw), _addr(db), _addr(part))
+    return dx, dw, db
+
+
+# ------------------------------------------- gradient norm and clipping (csrc/grads.hip) --------
+def _dense(t):
+    """whether t's elements fill one run of memory (in any order of its axes)"""
+    if t.is_contiguous():
+        return True
+    n = 1
+    for size, stride in sorted(((a, b) for a, b in zip(t.shape, t.stride()) if a != 1),
+                               key=lambda d: d[1]):
+        if stride != n:
+            return False
+        n *= size
+    return True
+
+
+def _grad_list(grads, what, disjoint):
+    grads = list(grads)
+    if not grads:
+        raise ValueError(f"{what}: no tensors")
+    _lib.require_gpu(*grads)
+    for t in grads:
+        if t.layout != torch.strided or t.dtype not in TYPES or not _dense(t):
+            raise ValueError(f"{what}: dense fp32, bf16 or fp16 tensors, got {t.dtype} "
+                             f"{tuple(t.shape)} with strides {t.stride() if t.layout == torch.strided else t.layout}")
+        if t.device != grads[0].device:
+            raise ValueError(f"{what}: tensors on {grads[0].device} and {t.device}")
+    n = [t.numel() for t in grads]
+    at = [t.data_ptr() for t in grads]
+    if disjoint:
+        end = 0
+        for a, b in sorted((p, p + k * t.element_size()) for p, k, t in zip(at, n, grads) if k):
+            if a < end:
+                raise ValueError(f"{what}: two of the tensors share memory")
+            end = b
+    k = len(grads)
+    return (grads, (ctypes.c_void_p * k)(*at), (ctypes.c_int64 * k)(*n),
+            (ctypes.c_int32 * k)(*[TYPES[t.dtype] for t in grads]))
+
+
+def _sumsq(grads, at, n, types):
+    dev = grads[0].device
+    parts = _lib.load().prfl_grads_parts(n, len(grads))
+    ws = torch.empty(parts + 1, dtype=torch.float64, device=dev)
+    _lib.call_on(dev, "prfl_grads_sumsq", at, n, types, len(grads), ws.data_ptr(), parts,
+                 ws.data_ptr() + 8 * parts)
+    return ws[parts:]
+
+
+def grads_sumsq(grads):
+    """Sum of the squares of all elements of a list of dense fp32 / bf16 / fp16 tensors: fp64 [1] on
+    their device.  (Ranks that hold shards add theirs, then clip_grads(sumsq=...).)"""
+    return _sumsq(*_grad_list(grads, "grads_sumsq", False))
+
+
+def clip_grads(grads, max_norm, eps=1e-6, out=None, sumsq=None):
+    """Scale the tensors by min(1, max_norm / (norm + eps)), norm their global L2 norm (or
+    sqrt(sumsq) where that is given); in place, or into `out`, a list of tensors of the same shapes
+    and one type.  Returns the norm before clipping, fp32 0-dim on the device (nothing waits)."""
+    if not max_norm >= 0 or not eps >= 0:
+        raise ValueError(f"clip_grads: max_norm and eps are not negative, got {max_norm}, {eps}")
+    grads = list(grads)
+    dst, otype = None, -1
+    if out is not None:
+        out = list(out)
+        if len(out) != len(grads) or any(o.shape != g.shape or o.stride() != g.stride()
+                                         or o.dtype != out[0].dtype for o, g in zip(out, grads)):
+            raise ValueError("clip_grads: out has the gradients' shapes and strides, and one type")
+        both, at, n, types = _grad_list(grads + out, "clip_grads", True)
+        k = len(grads)
+        otype = TYPES[out[0].dtype]
+        dst = (ctypes.c_void_p * k)(*at[k:])
+        lists = (grads, at, n, types)       # the first k of each
+    else:
+        lists = _grad_list(grads, "clip_grads", True)
+    dev = grads[0].device
+    if sumsq is None:
+        sumsq = _sumsq(*lists)
+    elif sumsq.dtype != torch.float64 or sumsq.numel() != 1 or sumsq.device != dev:
+        raise ValueError("clip_grads: sumsq is one fp64 value on the gradients' device")
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    _lib.call_on(dev, "prfl_grads_clip", lists[1], dst, lists[2], lists[3], len(grads), otype,
+                 sumsq.data_ptr(), max_norm, eps, norm.data_ptr())
+    return norm
+
+
+# ------------------------------------------------------------ microscaled fp4 (csrc/mxfp4.hip) --
+def _mx_shape(rows, cols):
+    return -(-rows // 64), -(-cols // 128)
+
+
+def quant_mxfp4(x):
+    """x [M, K] (fp32 / bf16 / fp16, row-strided) -> (q uint8 [M/64, K/128, 4, 64, 16], s uint8
+    [M/64, K/128, 64, 4]): e2m1 codes and e8m0 scales in the tiled layout of include/prfl_hip.h."""
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"quant_mxfp4: [M, K] with K >= 1, got {tuple(x.shape)}")
+    dev = _one_device("quant_mxfp4", x)
+    xt = _type(x.dtype, "quant_mxfp4")
+    M, K = x.shape
+    x = _rows(x, K)
+    G, S = _mx_shape(M, K)
+    q = torch.empty(G, S, 4, 64, 16, dtype=torch.uint8, device=dev)
+    s = torch.empty(G, S, 64, 4, dtype=torch.uint8, device=dev)
+    _lib.call_on(dev, "prfl_quant_mxfp4", x.data_ptr(), xt, x.stride(0), M, K, q.data_ptr(),
+                 s.data_ptr())
+    return q, s
+
+
+def _mx_check(what, q, s, rows, cols):
+    if cols < 1 or rows < 0:
+        raise ValueError(f"{what}: a [{rows}, {cols}] matrix")
+    G, S = _mx_shape(rows, cols)
+    if (q.shape != (G, S, 4, 64, 16) or s.shape != (G, S, 64, 4) or q.dtype != torch.uint8
+            or s.dtype != torch.uint8 or not q.is_contiguous() or not s.is_contiguous()):
+        raise ValueError(f"{what}: a tiled [{rows}, {cols}] matrix has contiguous uint8 q "
+                         f"{(G, S, 4, 64, 16)} and s {(G, S, 64, 4)}, got {tuple(q.shape)} and "
+                         f"{tuple(s.shape)}")
+
+
+def dequant_mxfp4(q, s, rows, cols, out_dtype=BF16):
+    """The values of quant_mxfp4's (q, s), [rows, cols] in bf16 (exact) or fp32."""
+    dev = _one_device("dequant_mxfp4", q, s)
+    _mx_check("dequant_mxfp4", q, s, rows, cols)
+    if out_dtype not in (BF16, torch.float32):
+        raise ValueError(f"dequant_mxfp4: bf16 or fp32, got {out_dtype}")
+    out = torch.empty(rows, cols, dtype=out_dtype, device=dev)
+    _lib.call_on(dev, "prfl_dequant_mxfp4", q.data_ptr(), s.data_ptr(), rows, cols, out.data_ptr(),
+                 int(out_dtype == torch.float32), cols)
+    return out
+
+
+def linear_mxfp4(x, wq, ws, out_features, bias=None):
+    """y [..., N] bf16 = x W^T + bias on the block-scaled MFMA: x [..., K] (fp32 / bf16 / fp16) is
+    quantised to microscaled fp4 in the call, (wq, ws) = quant_mxfp4(W [N, K]), bias bf16 [N]."""
+    if x.dim() < 1 or x.shape[-1] < 1 or out_features < 1:
+        raise ValueError(f"linear_mxfp4: x is [..., K], got {tuple(x.shape)} to {out_features}")
+    K, N = x.shape[-1], out_features
+    dev = _one_device("linear_mxfp4", x, wq, ws, bias)
+    _mx_check("linear_mxfp4", wq, ws, N, K)
+    if bias is not None and (bias.dtype != BF16 or bias.shape != (N,) or not bias.is_contiguous()):
+        raise ValueError(f"linear_mxfp4: a contiguous bf16 bias of [{N}]")
+    _type(x.dtype, "linear_mxfp4")
+    x2 = _rows(x, K)
+    M = x2.shape[0]
+    y = torch.empty(*x.shape[:-1], N, dtype=BF16, device=dev)
+    if M:
+        xq, xs = quant_mxfp4(x2)
+        _lib.call_on(dev, "prfl_gemm_mxfp4", xq.data_ptr(), xs.data_ptr(), wq.data_ptr(),
+                     ws.data_ptr(), _addr(bias), y.data_ptr(), N, M, N, K)
+    return y
+
+
+def linear_mxfp4_dx(dy, wq, ws, in_features):
+    """dx [..., K] bf16 = dy W of linear_mxfp4, x's quantisation taken as the identity: W is read
+    back to bf16 (exact) and multiplied on the bf16 MFMA.  dy [..., N] is taken in bf16."""
+    N, K = dy.shape[-1], in_features
+    dev = _one_device("linear_mxfp4_dx", dy, wq, ws)
+    _mx_check("linear_mxfp4_dx", wq, ws, N, K)
+    _type(dy.dtype, "linear_mxfp4_dx")
+    d = _rows(dy, N).to(BF16)
+    M, Np, Kp = d.shape[0], -(-N // 8) * 8, -(-K // 8) * 8
+    if M == 0:
+        return torch.empty(*dy.shape[:-1], K, dtype=BF16, device=dev)
+    # the bf16 product takes extents in eights: padding rows and columns of W read back as zeros
+    w = dequant_mxfp4(wq, ws, Np, Kp)
+    if Np != N:
+        d = torch.nn.functional.pad(d, (0, Np - N))
+    elif d.stride(0) % 8 or d.data_ptr() % 16:
+        d = d.clone(memory_format=torch.contiguous_format)
+    with torch.cuda.device(dev):
+        dx = linear_dx(d, w)
+    if Kp != K:
+        dx = dx[:, :K].contiguous()
+    return dx.view(*dy.shape[:-1], K)
 
 
 def prof_enable(on=True):

@@ -31,6 +31,8 @@
 * ``clip_grad_norm_`` — global L2 norm over all grads and in-place scaling by
                         min(1, max_norm/(norm+1e-6)) (`train_prfl.py:825,972`), with the clip
                         coefficient kept on the device (no host synchronisation).
+* ``clip_grads_``     — the same over fp32 / bf16 / fp16 gradients in a launch per 128 tensors, the
+                        squares summed in 64 bits and a fixed order (csrc/grads.hip).
 """
 import weakref
 
@@ -485,3 +487,14 @@ def clip_grad_norm_(params, max_norm=1.0, eps=1e-6):
     for g in grads:
         ops.scale_(g, coef)
     return total[0]
+
+
+@torch.no_grad()
+def clip_grads_(params, max_norm=1.0, eps=1e-6):
+    """clip_grad_norm_ over many tensors at once: gradients of any of the three types, the same bits
+    every time, nothing written when the norm is within max_norm.  Returns the norm before clipping
+    as a 0-dim device tensor (no host sync).  Parameters without a gradient are passed over."""
+    grads = [p.grad for p in params if p.grad is not None]
+    if not grads:
+        return torch.zeros(())
+    return ops.clip_grads(grads, max_norm, eps)

@@ -271,6 +271,62 @@ int prfl_gemm_fp8(const void* A, int64_t lda, const float* sa, const void* B, in
                   int epilogue, const void* bias, const float* gate, const void* res, int64_t ldr,
                   int res_bf16, void* aux, int64_t ldaux, void* stream);
 
+/* ---- layer norm over the last axis ---------------------------------------------------------
+ * The general form beside prfl_ln_mod_*: nn.LayerNorm (img_emb's, model.py:360-372; norm3,
+ * model.py:304-306) with any width C <= 16384, row stride and type, and its whole backward.
+ *   y = (x - mean) * rstd * w + b,  rstd = 1 / sqrt(var + eps), var over C elements (not C - 1)
+ * x_type / y_type / w_type: 0 fp32, 1 bf16, 2 fp16.  w and b (each may be NULL, both w_type) are
+ * contiguous, x / y rows have unit column stride.  mean / rstd [rows] fp32 are written for the
+ * backward.  Statistics and sums are fp32 (or more); y is rounded once. */
+int prfl_layer_norm_fwd(const void* x, int x_type, int64_t ldx, int64_t rows, int64_t C,
+                        const void* w, const void* b, int w_type, float eps, void* y, int y_type,
+                        int64_t ldy, float* mean, float* rstd, void* stream);
+/* dx (x_type) and, where the pointer is not NULL, dw = sum dy * xhat and db = sum dy (fp32 [C]).
+ * part: caller-owned fp32 workspace of prfl_layer_norm_parts(rows, C, x_type) * C elements for
+ * each of dw and db that is asked for (may be NULL if neither is).  dx may be NULL.  The sums run
+ * in a fixed order (no atomics).  rows == 0 writes dw and db as zeros. */
+int prfl_layer_norm_bwd(const void* dy, int y_type, int64_t lddy, const void* x, int x_type,
+                        int64_t ldx, const float* mean, const float* rstd, int64_t rows, int64_t C,
+                        const void* w, int w_type, void* dx, int64_t lddx, float* dw, float* db,
+                        float* part, void* stream);
+int64_t prfl_layer_norm_parts(int64_t rows, int64_t C, int x_type);
+
+/* ---- gradient norm and clipping over many tensors -------------------------------------------
+ * transformer.clip_grad_norm_ (train_prfl.py:825, :972) in a launch per 128 tensors instead of two
+ * per tensor.  grads / n / type are HOST arrays of count entries (device addresses, elements,
+ * 0 fp32 / 1 bf16 / 2 fp16); the lists travel in kernel arguments, so nothing is copied to the
+ * device and a captured graph replays them.  Entries of 0 elements are skipped.
+ * prfl_grads_sumsq: sumsq[0] (device, fp64) = sum of all squares, in 64 bits and a fixed order;
+ * part: workspace of prfl_grads_parts(n, count) doubles.  Ranks that hold shards of the gradients
+ * add their sumsq before the clip. */
+int64_t prfl_grads_parts(const int64_t* n, int64_t count);
+int prfl_grads_sumsq(const void* const* grads, const int64_t* n, const int32_t* type, int64_t count,
+                     double* part, int64_t parts, double* sumsq, void* stream);
+/* g *= min(1, max_norm / (norm + eps)), norm = sqrt(sumsq[0]); norm[0] (fp32, may be NULL) gets it.
+ * out == NULL: in place (nothing is touched when the factor is 1), else out[i] (out_type, as many
+ * elements) = the clipped gradient.  A NaN norm makes every gradient NaN. */
+int prfl_grads_clip(const void* const* grads, void* const* out, const int64_t* n,
+                    const int32_t* type, int64_t count, int out_type, const double* sumsq,
+                    float max_norm, float eps, float* norm, void* stream);
+
+/* ---- microscaled fp4 (OCP MX: e2m1 elements, one e8m0 scale per 32 of a row) ------------------
+ * Beside the e4m3 path: nn.Linear forwards of a frozen trunk (the latent reward model,
+ * train_prfl.py:217-266) with the weight in 4.25 bits an element.  The reference is bf16 only.
+ *   e = max(floor(log2(max |v|)) - 2, -127) per block;  code = v / 2^e to the nearest e2m1 value,
+ *   ties to even, saturating at 6;  a block with a NaN or an infinity reads back as NaN (scale 0xff)
+ * Tiled layout, R = ceil(rows / 64), S = ceil(K / 128):  q [R][S][4][64][16] bytes, s [R][S][64][4]
+ * bytes.  Element (row, k): piece (row / 64, k / 128), operand u = 2 * (row % 64 / 32) + k % 128 / 64,
+ * lane l = 32 * (k % 64 / 32) + row % 32; its code is nibble k % 2 of byte k % 32 / 2 of
+ * q[..][u][l], its scale s[..][l][u].  Padding rows and columns are zeros (codes and scales). */
+int prfl_quant_mxfp4(const void* x, int x_type, int64_t ldx, int64_t M, int64_t K, void* q, void* s,
+                     void* stream);
+int prfl_dequant_mxfp4(const void* q, const void* s, int64_t M, int64_t K, void* out, int out_f32,
+                       int64_t ldo, void* stream);
+/* y [M][N] bf16 = x W^T + bias (bf16 [N] or NULL): x [M][K] and W [N][K] both tiled, products on
+ * the block-scaled MFMA, fp32 sums, one rounding. */
+int prfl_gemm_mxfp4(const void* xq, const void* xs, const void* wq, const void* ws, const void* bias,
+                    void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, void* stream);
+
 /* ---- FlowUniPC sampler update (bh2, order <= 2, x0-prediction) ----------------------------
  * Replaces the element-wise body of FlowUniPCMultistepScheduler.step
  * (diffusers_lite/wan/utils/fm_solvers_unipc.py:655-739: convert_model_output :321, UniC
