@@ -782,18 +782,11 @@ __device__ __forceinline__ bool epi4_full(const GemmArgs& g, int m0, int n0, int
 #ifndef GEMM4_PREWAIT
 #define GEMM4_PREWAIT 1
 #endif
-// 1: every non-MFMA instruction of the four-wave loop between two MFMAs, as hipBLASLt's TN
-// loop places them (one LDS-DMA piece after MFMA 0, the A / B fragment reads after MFMAs 1 / 2 of
-// each 8-MFMA chunk) instead of a [piece, reads, 8 MFMAs] burst: bit-identical, forward +0.2-1.7 %,
-// dX +1.1-6.7 % on the 720p shapes (profiles/r04_ab_gemm_il.txt)
-#ifndef GEMM4_IL
-#define GEMM4_IL 1
-#endif
-// the same placement in the 32x32x16 weight-gradient kernel: dW +5.3-9.5 %, bit-identical
-// (profiles/r04_ab_gemm4x_il.txt)
-#ifndef GEMM4X_IL
-#define GEMM4X_IL 1
-#endif
+// Placement in the four-wave loops: a chunk has 8 MFMAs of 16 cycles (4 of 32 in gemm4x_kernel) and
+// three other issues -- two fragment reads and one LDS-DMA piece.  With one wave per SIMD nothing
+// else fills the matrix pipe while such an issue holds the port, so they are spread evenly, a read
+// after every second MFMA and the piece after the sixth (one after each of gemm4x_kernel's first
+// three): each has at least a whole MFMA's cycles to issue under.  Same MFMAs in the same order.
 // AGPR-accumulator MFMA as inline asm ("+a" keeps hipcc from moving the accumulators to VGPRs)
 __device__ __forceinline__ void mfma16(f32x4& acc, bf16x8 b, bf16x8 a) {
   asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc) : "v"(b), "v"(a));
@@ -801,8 +794,7 @@ __device__ __forceinline__ void mfma16(f32x4& acc, bf16x8 b, bf16x8 a) {
 
 // A64: a K-major A operand staged 64 deep.  A 32-deep K-major slice moves each A row as a 64-B
 // run (one LDS-DMA piece = 16 rows x 64 B = 16 half cache lines); staged 64 deep, a piece is 8
-// rows x 128 B = 8 whole lines, as hipBLASLt's MT256x256x64 TN loop fetches its operands.  The A
-// operand gets its own ring of three 64-deep slots (3 x 32 KiB) beside the B operand's ring of
+// rows x 128 B = 8 whole lines.  The A operand gets its own ring of three 64-deep slots (3 x 32 KiB) beside the B operand's ring of
 // four 32-deep slots (4 x 16 KiB): exactly the 160 KiB of LDS.  The 32-deep step schedule is
 // unchanged (one barrier per 32-deep sub-slice, fragments of sub-slice j+1 read during the MFMAs
 // of sub-slice j, 8 DMA pieces per wave per step, vmcnt(8)); A slice J (sub-slices 2J, 2J+1) is
@@ -826,8 +818,7 @@ constexpr int A64SLOT = 32768;
 // the DMA runs 14 % faster and one without its vmcnt waits no faster (profiles/r05_ab_gemm_diag.txt):
 // what the pieces cost is neither the data's arrival nor the four waves' collision.  Moving every
 // wave's piece to MFMA gap 3, 5 or 7 of the chunk ties within 0.5 %, profiles/r05_ab_gemm_dgap.txt.
-// Also measured and dropped: the TN forward with B staged 64 deep too (hipBLASLt's operand format,
-// one ds_read_b128 per B fragment; A's three 64-deep slots + B's two fill the 160 KiB, so a B slice
+// Also measured and dropped: the TN forward with B staged 64 deep too (one ds_read_b128 per B fragment; A's three 64-deep slots + B's two fill the 160 KiB, so a B slice
 // has one step to land instead of two): bit-identical, 4-8 % SLOWER than the 32-deep forms,
 // profiles/r05_ab_gemm_b64.txt.)
 #ifndef GEMM4_DIAG
@@ -957,49 +948,21 @@ __global__ __launch_bounds__(256, 1) void gemm4w_kernel(GemmArgs g) {
     // over the slice (one wave per SIMD: nothing else fills the matrix pipe)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if (GEMM4_IL == 2) {    // the slice's 8 pieces in its first half, two per chunk
-        mfma16(acc[i][0], cb[0], ca[i]);
-        if (i < 4) piece(2 * i, jd, sd);
-        mfma16(acc[i][1], cb[1], ca[i]);
-        if (i < 4) piece(2 * i + 1, jd, sd);
-        mfma16(acc[i][2], cb[2], ca[i]);
-        __builtin_amdgcn_sched_barrier(0);
-        na[i] = read_frag4<A_KC>(st, wm * 128 + i * 16, lane);
-        __builtin_amdgcn_sched_barrier(0);
-        mfma16(acc[i][3], cb[3], ca[i]);
-        __builtin_amdgcn_sched_barrier(0);
-        nb[i] = read_frag4<B_KC>(st + HALF4, wn * 128 + i * 16, lane);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int jj = 4; jj < 8; ++jj) mfma16(acc[i][jj], cb[jj], ca[i]);
-        __builtin_amdgcn_sched_barrier(0);
-        continue;
-      }
-      if (GEMM4_IL) {
-        // hipBLASLt's placement (its TN loop, disassembled): every non-MFMA instruction sits
-        // BETWEEN two MFMAs, so the matrix pipe has the next product queued behind it
-        mfma16(acc[i][0], cb[0], ca[i]);
-        piece(i, jd, sd);
-        mfma16(acc[i][1], cb[1], ca[i]);
-        __builtin_amdgcn_sched_barrier(0);
-        na[i] = read_frag4<A_KC>(st, wm * 128 + i * 16, lane);
-        __builtin_amdgcn_sched_barrier(0);
-        mfma16(acc[i][2], cb[2], ca[i]);
-        __builtin_amdgcn_sched_barrier(0);
-        nb[i] = read_frag4<B_KC>(st + HALF4, wn * 128 + i * 16, lane);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int jj = 3; jj < 8; ++jj) mfma16(acc[i][jj], cb[jj], ca[i]);
-        __builtin_amdgcn_sched_barrier(0);
-        continue;
-      }
-      piece(i, jd, sd);
+      mfma16(acc[i][0], cb[0], ca[i]);
+      mfma16(acc[i][1], cb[1], ca[i]);
+      __builtin_amdgcn_sched_barrier(0);
       na[i] = read_frag4<A_KC>(st, wm * 128 + i * 16, lane);
+      __builtin_amdgcn_sched_barrier(0);
+      mfma16(acc[i][2], cb[2], ca[i]);
+      mfma16(acc[i][3], cb[3], ca[i]);
+      __builtin_amdgcn_sched_barrier(0);
       nb[i] = read_frag4<B_KC>(st + HALF4, wn * 128 + i * 16, lane);
-#pragma unroll
-      for (int jj = 0; jj < 8; ++jj)   // AGPR accumulators: the MFMA as inline asm ("+a") keeps
-        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0"   // hipcc from switching them to
-                     : "+a"(acc[i][jj]) : "v"(cb[jj]), "v"(ca[i]));   // VGPRs and spilling
+      __builtin_amdgcn_sched_barrier(0);
+      mfma16(acc[i][4], cb[4], ca[i]);
+      mfma16(acc[i][5], cb[5], ca[i]);
+      piece(i, jd, sd);
+      mfma16(acc[i][6], cb[6], ca[i]);
+      mfma16(acc[i][7], cb[7], ca[i]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -1017,20 +980,23 @@ __global__ __launch_bounds__(256, 1) void gemm4w_kernel(GemmArgs g) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       mfma16(acc[i][0], cb[0], ca[i]);
-      if (!(GEMM4_DIAG & 2)) {
-        if (i < 4) piece_a64(i, J, hh, sa);
-        else piece_b(i - 4, jb, sb);
-      }
       mfma16(acc[i][1], cb[1], ca[i]);
       __builtin_amdgcn_sched_barrier(0);
       na[i] = (GEMM4_DIAG & 4) ? ca[i] : read_frag_a64(ra, hr, wm * 128 + i * 16, lane);
       __builtin_amdgcn_sched_barrier(0);
       mfma16(acc[i][2], cb[2], ca[i]);
+      mfma16(acc[i][3], cb[3], ca[i]);
       __builtin_amdgcn_sched_barrier(0);
       nb[i] = (GEMM4_DIAG & 4) ? cb[i] : read_frag4<B_KC>(rb, wn * 128 + i * 16, lane);
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int jj = 3; jj < 8; ++jj) mfma16(acc[i][jj], cb[jj], ca[i]);
+      mfma16(acc[i][4], cb[4], ca[i]);
+      mfma16(acc[i][5], cb[5], ca[i]);
+      if (!(GEMM4_DIAG & 2)) {
+        if (i < 4) piece_a64(i, J, hh, sa);
+        else piece_b(i - 4, jb, sb);
+      }
+      mfma16(acc[i][6], cb[6], ca[i]);
+      mfma16(acc[i][7], cb[7], ca[i]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -1322,32 +1288,21 @@ __global__ __launch_bounds__(256, 1) void gemm4x_kernel(GemmArgs g) {
 #pragma unroll
     for (int c = 0; c < 8; ++c) {
       const int s = c >> 2, i = c & 3;
-      if (GEMM4X_IL) {       // the four-wave kernel's GEMM4_IL placement: each between two MFMAs
-        auto mf = [&](int jj) {
-          asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0"
-                       : "+a"(acc[i][jj]) : "v"(cb[4 * s + jj]), "v"(ca[c]));
-        };
-        mf(0);
-        piece(c, jd, sd);
-        mf(1);
-        __builtin_amdgcn_sched_barrier(0);
-        na[c] = read_frag32<A_KC>(st, wm * 128 + (c & 3) * 32, c >> 2, lane);
-        __builtin_amdgcn_sched_barrier(0);
-        mf(2);
-        __builtin_amdgcn_sched_barrier(0);
-        nb[c] = read_frag32<B_KC>(st + HALF4, wn * 128 + (c & 3) * 32, c >> 2, lane);
-        __builtin_amdgcn_sched_barrier(0);
-        mf(3);
-        __builtin_amdgcn_sched_barrier(0);
-        continue;
-      }
-      piece(c, jd, sd);
-      na[c] = read_frag32<A_KC>(st, wm * 128 + (c & 3) * 32, c >> 2, lane);
-      nb[c] = read_frag32<B_KC>(st + HALF4, wn * 128 + (c & 3) * 32, c >> 2, lane);
-#pragma unroll
-      for (int jj = 0; jj < 4; ++jj)   // D = B . A^T: lanes own consecutive n of one row m
+      auto mf = [&](int jj) {   // D = B . A^T: lanes own consecutive n of one row m
         asm volatile("v_mfma_f32_32x32x16_bf16 %0, %1, %2, %0"
                      : "+a"(acc[i][jj]) : "v"(cb[4 * s + jj]), "v"(ca[c]));
+      };
+      mf(0);
+      __builtin_amdgcn_sched_barrier(0);
+      na[c] = read_frag32<A_KC>(st, wm * 128 + (c & 3) * 32, c >> 2, lane);
+      __builtin_amdgcn_sched_barrier(0);
+      mf(1);
+      __builtin_amdgcn_sched_barrier(0);
+      nb[c] = read_frag32<B_KC>(st + HALF4, wn * 128 + (c & 3) * 32, c >> 2, lane);
+      __builtin_amdgcn_sched_barrier(0);
+      mf(2);
+      piece(c, jd, sd);
+      mf(3);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
