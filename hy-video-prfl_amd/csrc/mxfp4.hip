@@ -167,49 +167,342 @@ __device__ __forceinline__ void store4(const MxArgs& a, int64_t m, int n, const 
   }
 }
 
-// 64 columns x 64 rows of y per wave, the operands straight from memory
-__global__ __launch_bounds__(NT) void mx_gemm_kernel(MxArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int gn = (a.N + 63) / 64;
-  const int64_t gm = (a.M + 63) / 64, unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (unit >= gn * gm) return;
-  const int64_t n = unit % gn, m = unit / gn;
-  const u32x4* w = (const u32x4*)(a.wq + n * a.steps * PIECE) + lane;
-  const u32x4* x = (const u32x4*)(a.xq + m * a.steps * PIECE) + lane;
-  const uint32_t* sw = (const uint32_t*)(a.ws + n * a.steps * PIECE_S) + lane;
-  const uint32_t* sx = (const uint32_t*)(a.xs + m * a.steps * PIECE_S) + lane;
-  f32x16 acc[2][2];
+// tile of workgroup bid: every eighth workgroup runs on the same XCD, so XCD k gets the k-th eighth of
+// the tiles, and within it 8 tile rows advance over the tile columns together (their operands
+// meet in that XCD's L2)
+__device__ __forceinline__ void tile_of(int bid, int ntm, int ntn, int& tm, int& tn) {
+  const int all = ntm * ntn, xcd = bid & 7, q = all >> 3, r = all & 7;
+  const int w = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (bid >> 3);
+  const int g = w / (8 * ntn), rows = min(ntm - g * 8, 8), in = w - g * 8 * ntn;
+  tm = g * 8 + in % rows;
+  tn = in / rows;
+}
+
+// LDS-DMA of 4 B a lane (lane i lands at m0 + 4 i) from a buffer at voff + soff
+__device__ __forceinline__ void dma4_step(i32x4 srd, uint32_t voff, uint32_t soff) {
+  asm volatile("buffer_load_dword %0, %1, %2 offen lds"
+               :: "v"(voff), "s"(srd), "s"(__builtin_amdgcn_readfirstlane(soff)) : "memory");
+}
+
+// Few rows (M <= 32 MT, MT 1 or 2): 32 columns of y per workgroup, its 16 waves taking every 16th step of
+// 128 along K, their partial sums joined through LDS in wave order.  W is read once, in lane order, with up to
+// four steps of it in flight per wave: the time is W's bytes.  FUSED: x comes as it is, at most 1024 blocks
+// of 32, and every workgroup quantises all of it, a block per thread, into LDS ([block][row]: rows beyond M
+// take no room) -- one launch instead of two, while W's first loads are under way; else x comes tiled.
+template <typename T, int N>
+__device__ __forceinline__ void load_block(const T* p, int n, float (&v)[N]) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int c = 0; c < N; c += 8) {
+    if (n >= c + 8) {
+      const typename Loaded<T, 8>::vec t = *(const typename Loaded<T, 8>::at*)(p + c);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) acc[i][j] = (f32x16)(0.f);
-  for (int k = 0; k < a.steps; ++k) {
-    u32x4 wv[4], xv[4];
+      for (int i = 0; i < 8; ++i) v[c + i] = (float)t[i];
+    } else {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      wv[u] = w[k * 256 + u * 64];
-      xv[u] = x[k * 256 + u * 64];
+      for (int i = 0; i < 8; ++i) v[c + i] = c + i < n ? (float)p[c + i] : 0.f;
     }
-    const uint32_t s0 = sw[k * 64], s1 = sx[k * 64];
-    acc[0][0] = mfma4<0, 0>(wv[0], xv[0], acc[0][0], s0, s1);
-    acc[0][1] = mfma4<0, 2>(wv[0], xv[2], acc[0][1], s0, s1);
-    acc[1][0] = mfma4<2, 0>(wv[2], xv[0], acc[1][0], s0, s1);
-    acc[1][1] = mfma4<2, 2>(wv[2], xv[2], acc[1][1], s0, s1);
-    acc[0][0] = mfma4<1, 1>(wv[1], xv[1], acc[0][0], s0, s1);
-    acc[0][1] = mfma4<1, 3>(wv[1], xv[3], acc[0][1], s0, s1);
-    acc[1][0] = mfma4<3, 1>(wv[3], xv[1], acc[1][0], s0, s1);
-    acc[1][1] = mfma4<3, 3>(wv[3], xv[3], acc[1][1], s0, s1);
   }
+}
+constexpr int ROWS_WAVES = 16, ROWS_FUSED = 64 * ROWS_WAVES;
+
+template <typename T, int MT, bool FUSED>
+__global__ __launch_bounds__(64 * ROWS_WAVES) void mx_rows_kernel(MxArgs a, const T* __restrict__ x, int64_t ldx,
+                                                                  int K) {
+  __shared__ __attribute__((aligned(16))) float part[ROWS_WAVES * 1024];
+  __shared__ __attribute__((aligned(16))) u32x4 lx[FUSED ? ROWS_FUSED : 1];
+  __shared__ uint8_t lsx[FUSED ? ROWS_FUSED : 1];
+  const int lane = threadIdx.x & 63, row = lane & 31, blk = lane >> 5;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nt = blockIdx.x, steps = a.steps, M = (int)a.M;
+  const uint8_t* w = a.wq + (int64_t)(nt >> 1) * steps * PIECE + (nt & 1) * 2048 + lane * 16;
+  const uint8_t* sw = a.ws + (int64_t)(nt >> 1) * steps * PIECE_S + lane * 4;
+  constexpr int AHEAD = 4;
+  f32x16 acc[MT];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int m = 0; m < MT; ++m) acc[m] = (f32x16)(0.f);
+
+  u32x4 wv[AHEAD][2];
+  uint32_t sv[AHEAD];
+  auto load_w = [&](int k0) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int u = 0; u < AHEAD; ++u) {
+      const int k = k0 + u * ROWS_WAVES;
+      if (k >= steps) continue;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) wv[u][h] = *(const u32x4*)(w + (int64_t)k * PIECE + h * 1024);
+      sv[u] = *(const uint32_t*)(sw + (int64_t)k * PIECE_S) >> (16 * (nt & 1));
+    }
+  };
+  load_w(wid);
+  if constexpr (FUSED) {
+    const int blocks = (K + 31) / 32, b = threadIdx.x / M, m = threadIdx.x - b * M;
+    if (b < blocks) {
+      float v[32];
+      load_block(x + m * ldx + b * 32, K - b * 32, v);
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) top = max(top, __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu);
+      const uint32_t byte = scale_byte(top);
+      u32x4 q;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float e[8] = {v[8 * i], v[8 * i + 1], v[8 * i + 2], v[8 * i + 3],
+                            v[8 * i + 4], v[8 * i + 5], v[8 * i + 6], v[8 * i + 7]};
+        q[i] = byte == 255 ? 0u : pack8(e, scale_value(byte));
+      }
+      lx[b * M + m] = q;
+      lsx[b * M + m] = (uint8_t)byte;
+    }
+    __syncthreads();
+  }
+  for (int k0 = wid; k0 < steps; k0 += AHEAD * ROWS_WAVES) {
+    if (k0 != wid) load_w(k0);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int k = k0 + u * ROWS_WAVES;
+      if (k >= steps) break;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        u32x4 xv[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+        uint32_t sx = 0;
+        if constexpr (FUSED) {
+          const int blocks = (K + 31) / 32;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int b = k * 4 + h * 2 + blk;
+            if (row < M && b < blocks) {
+              xv[h] = lx[b * M + row];
+              sx |= (uint32_t)lsx[b * M + row] << (8 * h);
+            }
+          }
+        } else if (m * 32 + row < M) {
+          const uint8_t* xp = a.xq + (int64_t)k * PIECE + m * 2048 + lane * 16;
+          xv[0] = *(const u32x4*)xp;
+          xv[1] = *(const u32x4*)(xp + 1024);
+          sx = *(const uint32_t*)(a.xs + (int64_t)k * PIECE_S + lane * 4) >> (16 * m);
+        }
+        acc[m] = mfma4<0, 0>(wv[u][0], xv[0], acc[m], sv[u], sx);
+        acc[m] = mfma4<1, 1>(wv[u][1], xv[1], acc[m], sv[u], sx);
+      }
+    }
+  }
+  // register 4 q + c of lane l is column 8 q + 4 (l / 32) + c of row l % 32
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    if (m) __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 v = {acc[m][4 * q], acc[m][4 * q + 1], acc[m][4 * q + 2], acc[m][4 * q + 3]};
+      *(f32x4*)(part + wid * 1024 + q * 256 + lane * 4) = v;
+    }
+    __syncthreads();
+    const int t = threadIdx.x, l = (t >> 2) & 63, mm = m * 32 + (l & 31);
+    const int n = nt * 32 + 8 * (t >> 8) + 4 * (l >> 5) + (t & 3);
+    if (mm < M && n < a.N) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < ROWS_WAVES; ++i) s += part[i * 1024 + t];
+      a.y[mm * a.ldy + n] = f2bf(s + (a.bias ? bf2f(a.bias[n]) : 0.f));
+    }
+  }
+}
+
+// The tiled product: 64 WT x 64 WT of y per workgroup, four waves of 32 WT x 32 WT each.  Every step of
+// 128 columns (PIECE bytes a row piece) lands in a four-slot LDS ring by LDS-DMA, three steps ahead;
+// operands are in MFMA order already, so a piece is copied as it lies and every fragment is one
+// ds_read_b128 in lane order (no bank conflicts, no address arithmetic).
+//   step j: wait for the own DMA of step j+1 | barrier | DMA of step j+3 into the slot of step j-1
+//           | MFMAs of column half 0 beside the reads of half 1 | MFMAs of half 1 beside the reads
+//           of step j+1's half 0
+// RAW: step j+1 is read after the barrier that every wave passes with its part of it landed.  WAR: the
+// slot of step j-1 was read for MFMAs that precede this barrier in every wave.  Past the last
+// step the DMA fetches it again into a slot nobody reads, so the count is the same every step.
+template <int WT>
+__global__ __launch_bounds__(NT, WT == 4 ? 1 : 2) void mx_gemm_tile_kernel(MxArgs a) {
+  constexpr int OPB = WT * PIECE, OPS = WT * PIECE_S, SLOT = 2 * (OPB + OPS);
+  __shared__ __attribute__((aligned(16))) char smem[4 * SLOT];
+  const int lane = threadIdx.x & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wn = wid >> 1, wm = wid & 1;
+  int tm, tn;
+  tile_of(blockIdx.x, (int)((a.M + 64 * WT - 1) / (64 * WT)), (a.N + 64 * WT - 1) / (64 * WT), tm, tn);
+  const int steps = a.steps;
+
+  // DMA sources: a wave moves WT KiB of each operand and (WT 4: of both, WT 2: of one) 256 B of scales
+  // a step.  Row pieces past the matrix are clamped to its last (their results are not stored).
+  const int gn = (a.N + 63) / 64;
+  const int64_t gm = (a.M + 63) / 64;
+  const int own = WT == 4 ? wid : wid >> 1;             // row piece of the tile
+  const int part = WT == 4 ? 0 : (wid & 1) * 2048;
+  const int64_t pn = min(tn * WT + own, gn - 1), pm = min((int64_t)tm * WT + own, gm - 1);
+  const uint32_t bytes = (uint32_t)steps * PIECE;
+  const i32x4 srd_w = make_srd(a.wq + pn * steps * PIECE + part, bytes - part);
+  const i32x4 srd_x = make_srd(a.xq + pm * steps * PIECE + part, bytes - part);
+  const int64_t sn = min(tn * WT + (WT == 4 ? wid : wid & 1), gn - 1);
+  const int64_t sm = min((int64_t)tm * WT + (WT == 4 ? wid : wid & 1), gm - 1);
+  const i32x4 srd_sw = make_srd(a.ws + sn * steps * PIECE_S, (uint32_t)steps * PIECE_S);
+  const i32x4 srd_sx = make_srd(a.xs + sm * steps * PIECE_S, (uint32_t)steps * PIECE_S);
+  const uint32_t lds0 = lds_addr(smem);
+  unsigned keep = 0;
+  // DMA p of the step's DMAS
+  constexpr int DMAS = WT == 4 ? 10 : 5;
+  auto dma = [&](int p, int j) {
+    const uint32_t at = lds0 + (uint32_t)(j & 3) * SLOT, k = (uint32_t)min(j, steps - 1);
+    if (p < 2 * WT) {
+      const int op = p >= WT, i = p - op * WT;
+      if (i == 0) m0_set(at + op * OPB + wid * (WT * 1024), keep);
+      dma16_buf_m0(op ? srd_x : srd_w, lane * 16, k * PIECE, i);
+      if (i == WT - 1) m0_restore(keep);
+    } else {
+      const bool op = WT == 4 ? p == 2 * WT + 1 : wid >= 2;
+      const int i = WT == 4 ? wid : wid & 1;
+      m0_set(at + 2 * OPB + (op ? OPS : 0) + i * PIECE_S, keep);
+      dma4_step(op ? srd_sx : srd_sw, lane * 4, k * PIECE_S);
+      m0_restore(keep);
+    }
+  };
+
+  f32x16 acc[WT][WT];
+#pragma unroll
+  for (int i = 0; i < WT; ++i)
+#pragma unroll
+    for (int j = 0; j < WT; ++j) acc[i][j] = (f32x16)(0.f);
+  u32x4 f[2][2][WT];                     // [column half][W, x][tile]
+  uint32_t sc[2][2][WT / 2];             // [step parity][W, x][row piece]
+  // fragment r (< 2 WT) of half h, step j: the wave's row pieces start at wn (wm) * WT / 2
+  auto read = [&](int r, int h, int j) {
+    const int op = r >= WT, i = r - op * WT;
+    const char* st = smem + (j & 3) * SLOT + op * OPB + (op ? wm : wn) * (WT / 2) * PIECE;
+    f[h][op][i] = *(const u32x4*)(st + (i >> 1) * PIECE + ((i & 1) * 2 + h) * 1024 + lane * 16);
+  };
+  auto read_scales = [&](int par, int j) {
+#pragma unroll
+    for (int op = 0; op < 2; ++op)
+#pragma unroll
+      for (int i = 0; i < WT / 2; ++i)
+        sc[par][op][i] = *(const uint32_t*)(smem + (j & 3) * SLOT + 2 * OPB + op * OPS +
+                                            ((op ? wm : wn) * (WT / 2) + i) * PIECE_S + lane * 4);
+  };
+  // MFMA c of a half: tile pair (c / 4), then the four of its 2 x 2 tiles
+  auto product = [&](auto half, int par, int c) {
+    constexpr int H = half();
+    const int ii = c / 4 / (WT / 2), jj = c / 4 % (WT / 2), q = c & 3;
+    const uint32_t sw = sc[par][0][ii], sx = sc[par][1][jj];
+    f32x16& d = acc[2 * ii + (q >> 1)][2 * jj + (q & 1)];
+    const u32x4 w = f[H][0][2 * ii + (q >> 1)], x = f[H][1][2 * jj + (q & 1)];
+    if (q == 0) d = mfma4<H, H>(w, x, d, sw, sx);
+    else if (q == 1) d = mfma4<H, 2 + H>(w, x, d, sw, sx);
+    else if (q == 2) d = mfma4<2 + H, H>(w, x, d, sw, sx);
+    else d = mfma4<2 + H, 2 + H>(w, x, d, sw, sx);
+  };
+  auto step = [&](auto parity, int j) {
+    constexpr int P = parity();
+    if constexpr (DMAS == 10) asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(5)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < WT * WT; ++c) {
+      product(std::integral_constant<int, 0>(), P, c);
+      if (c < 2 * WT) read(c, 1, j);
+      if (c < DMAS) dma(c, j + 3);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int c = DMAS < WT * WT ? DMAS : WT * WT; c < DMAS; ++c) dma(c, j + 3);
+    read_scales(1 - P, j + 1);
+#pragma unroll
+    for (int c = 0; c < WT * WT; ++c) {
+      product(std::integral_constant<int, 1>(), P, c);
+      if (c < 2 * WT) read(c, 0, j + 1);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+#pragma unroll
+  for (int j = 0; j < 3; ++j)
+#pragma unroll
+    for (int p = 0; p < DMAS; ++p) dma(p, j);
+  if constexpr (DMAS == 10) asm volatile("s_waitcnt vmcnt(20)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int r = 0; r < 2 * WT; ++r) read(r, 0, 0);
+  read_scales(0, 0);
+  int j = 0;
+  for (; j + 1 < steps; j += 2) {
+    step(std::integral_constant<int, 0>(), j);
+    step(std::integral_constant<int, 1>(), j + 1);
+  }
+  if (j < steps) step(std::integral_constant<int, 0>(), j);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+  const int n0 = tn * 64 * WT + wn * 32 * WT;
+  const int64_t m0 = (int64_t)tm * 64 * WT + wm * 32 * WT;
+  // A tile whose columns are all there, with 16-B aligned rows, leaves through a wave-private LDS image (32 rows of the wave's
+  // columns at a time, 16 B of padding a row), so that a store instruction writes whole cache lines; in the
+  // MFMA layout it would write 64 pieces of 8 B.
+  constexpr int RB = 64 * WT, ROW = RB + 16, LPR = RB / 16, RPI = 64 / LPR;
+  static_assert(4 * WT * 32 * ROW <= 4 * SLOT, "the images reuse the ring");
+  if ((tn + 1) * 64 * WT <= a.N && a.ldy % 8 == 0 && ((uintptr_t)a.y & 15) == 0) {
+    typename Loaded<bf16, 4>::vec b[WT][4];
+#pragma unroll
+    for (int i = 0; i < WT; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float v[4] = {acc[i][j][4 * r], acc[i][j][4 * r + 1], acc[i][j][4 * r + 2], acc[i][j][4 * r + 3]};
-        store4(a, m * 64 + j * 32 + (lane & 31), (int)n * 64 + i * 32 + 8 * r + 4 * (lane >> 5), v);
+        b[i][r] = (typename Loaded<bf16, 4>::vec){};
+        if (a.bias) b[i][r] = *(const typename Loaded<bf16, 4>::at*)(a.bias + n0 + i * 32 + 8 * r + 4 * (lane >> 5));
+      }
+    __builtin_amdgcn_s_barrier();          // every wave's DMA has landed and its fragments are read
+    asm volatile("" ::: "memory");
+    char* img = smem + wid * (WT * 32 * ROW);
+#pragma unroll
+    for (int jj = 0; jj < WT; ++jj)
+#pragma unroll
+      for (int i = 0; i < WT; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          bf16x4 o;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[k] = f2bf(acc[i][jj][4 * r + k] + bf2f(b[i][r][k]));
+          *(bf16x4*)(img + (jj * 32 + (lane & 31)) * ROW + (i * 32 + 8 * r + 4 * (lane >> 5)) * 2) = o;
+        }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    bf16* const y0 = a.y + (m0 + lane / LPR) * a.ldy + n0 + (lane % LPR) * 8;
+#pragma unroll
+    for (int t = 0; t < WT * 32 / RPI; ++t)
+      if (m0 + t * RPI + lane / LPR < a.M)
+        *(u32x4*)(y0 + (int64_t)t * RPI * a.ldy) = *(const u32x4*)(img + (t * RPI + lane / LPR) * ROW + (lane % LPR) * 16);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < WT; ++i)
+#pragma unroll
+    for (int jj = 0; jj < WT; ++jj)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float v[4] = {acc[i][jj][4 * r], acc[i][jj][4 * r + 1], acc[i][jj][4 * r + 2], acc[i][jj][4 * r + 3]};
+        store4(a, m0 + jj * 32 + (lane & 31), n0 + i * 32 + 8 * r + 4 * (lane >> 5), v);
       }
 }
+
+constexpr int ROWS_MOST = 64;
+
+void launch_product(const MxArgs& a, hipStream_t st) {
+  const int64_t t256 = ((a.M + 255) / 256) * ((a.N + 255) / 256), t128 = ((a.M + 127) / 128) * ((a.N + 127) / 128);
+  const dim3 cols((unsigned)((a.N + 31) / 32));
+  if (a.M <= 32)
+    hipLaunchKernelGGL((mx_rows_kernel<bf16, 1, false>), cols, dim3(64 * ROWS_WAVES), 0, st, a, nullptr, 0, 0);
+  else if (a.M <= ROWS_MOST)
+    hipLaunchKernelGGL((mx_rows_kernel<bf16, 2, false>), cols, dim3(64 * ROWS_WAVES), 0, st, a, nullptr, 0, 0);
+  else if (t256 >= 432)
+    hipLaunchKernelGGL(mx_gemm_tile_kernel<4>, dim3((unsigned)t256), dim3(NT), 0, st, a);
+  else
+    hipLaunchKernelGGL(mx_gemm_tile_kernel<2>, dim3((unsigned)t128), dim3(NT), 0, st, a);
+}
+
+bool fused(int64_t M, int64_t K) { return M <= 32 && M * ((K + 31) / 32) <= ROWS_FUSED; }
 
 bool too_large(int64_t rows, int64_t cols) {       // pieces are counted in 31 bits
   return rows < 0 || cols < 1 || cols > (1 << 24) ||
@@ -272,9 +565,48 @@ extern "C" int prfl_gemm_mxfp4(const void* xq, const void* xs, const void* wq, c
   hipStream_t st = (hipStream_t)stream;
   MxArgs a{(const uint8_t*)wq, (const uint8_t*)ws, (const uint8_t*)xq, (const uint8_t*)xs,
            (const bf16*)bias, (bf16*)y, ldy, M, (int)N, (int)((K + 127) / 128)};
-  const int64_t units = ((M + 63) / 64) * ((N + 63) / 64);
   prfl_prof::begin(KID_GEMM, st);
-  hipLaunchKernelGGL(mx_gemm_kernel, dim3((unsigned)((units + 3) / 4)), dim3(NT), 0, st, a);
+  launch_product(a, st);
+  prfl_prof::set_work(2.0 * M * N * K);
+  prfl_prof::end(KID_GEMM, st);
+  PRFL_LAUNCH_CHECK();
+  return 0;
+}
+
+extern "C" int64_t prfl_linear_mxfp4_ws_bytes(int64_t M, int64_t K) {
+  if (M <= 0 || too_large(M, K) || fused(M, K)) return 0;
+  return ((M + 63) / 64) * ((K + 127) / 128) * (PIECE + PIECE_S);
+}
+
+extern "C" int prfl_linear_mxfp4(const void* x, int x_type, int64_t ldx, const void* wq, const void* ws,
+                                 const void* bias, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K,
+                                 void* work, int64_t work_bytes, void* stream) {
+  const int64_t need = prfl_linear_mxfp4_ws_bytes(M, K);
+  if (x_type < 0 || x_type > 2 || (M > 1 && ldx < 0) || work_bytes < need || (need && !work))
+    return (int)hipErrorInvalidValue;
+  if (need || M <= 0) {
+    uint8_t* xs = (uint8_t*)work + need / (PIECE + PIECE_S) * PIECE;
+    if (need)
+      if (int rc = prfl_quant_mxfp4(x, x_type, ldx, M, K, work, xs, stream)) return rc;
+    return prfl_gemm_mxfp4(work, xs, wq, ws, bias, y, ldy, M, N, K, stream);
+  }
+  if (too_large(M, K) || too_large(N, K) || N < 1 || N > (1 << 24) || (M > 1 && ldy < N) || !x || !wq || !ws || !y ||
+      ((uintptr_t)wq & 15) || ((uintptr_t)ws & 3))
+    return (int)hipErrorInvalidValue;
+  hipStream_t st = (hipStream_t)stream;
+  MxArgs a{(const uint8_t*)wq, (const uint8_t*)ws, nullptr, nullptr, (const bf16*)bias, (bf16*)y, ldy, M,
+           (int)N, (int)((K + 127) / 128)};
+  const dim3 cols((unsigned)((N + 31) / 32));
+  prfl_prof::begin(KID_GEMM, st);
+  if (x_type == 0)
+    hipLaunchKernelGGL((mx_rows_kernel<float, 1, true>), cols, dim3(64 * ROWS_WAVES), 0, st, a, (const float*)x, ldx,
+                       (int)K);
+  else if (x_type == 1)
+    hipLaunchKernelGGL((mx_rows_kernel<bf16, 1, true>), cols, dim3(64 * ROWS_WAVES), 0, st, a, (const bf16*)x, ldx,
+                       (int)K);
+  else
+    hipLaunchKernelGGL((mx_rows_kernel<_Float16, 1, true>), cols, dim3(64 * ROWS_WAVES), 0, st, a, (const _Float16*)x,
+                       ldx, (int)K);
   prfl_prof::set_work(2.0 * M * N * K);
   prfl_prof::end(KID_GEMM, st);
   PRFL_LAUNCH_CHECK();

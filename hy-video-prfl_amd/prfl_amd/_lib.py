@@ -86,6 +86,8 @@ SIGNATURES = {
     "prfl_grads_clip": [P, P, P, P, I64, I32, P, F32, F32, P, P],
     "prfl_quant_mxfp4": [P, I32, I64, I64, I64, P, P, P],
     "prfl_dequant_mxfp4": [P, P, I64, I64, P, I32, I64, P],
+    "prfl_linear_mxfp4_ws_bytes": [I64, I64],
+    "prfl_linear_mxfp4": [P, I32, I64, P, P, P, P, I64, I64, I64, I64, P, I64, P],
     "prfl_gemm_mxfp4": [P, P, P, P, P, P, I64, I64, I64, I64, P],
     "prfl_prof_enable": [I32],
     "prfl_prof_collect": [P, P, P, I32],
@@ -94,7 +96,8 @@ SIGNATURES = {
 
 # entries that return a value other than a hipError_t code
 RESTYPES = {"prfl_attn_fwd_ws_bytes": I64, "prfl_attn_vt_bytes": I64, "prfl_attn_fwd_fp8_ws_bytes": I64, "prfl_attn_bwd_ws_bytes": I64,
-            "prfl_layer_norm_parts": I64, "prfl_grads_parts": I64}
+            "prfl_layer_norm_parts": I64, "prfl_grads_parts": I64,
+            "prfl_linear_mxfp4_ws_bytes": I64}
 
 # kernel ids of the profiling hooks (csrc/common.h)
 KID = dict(gemm=0, attn_fwd=1, attn_fwd_short=2, attn_bwd_dkdv=3, attn_bwd_dq=4, ln=5, rms=6,
@@ -102,6 +105,9 @@ KID = dict(gemm=0, attn_fwd=1, attn_fwd_short=2, attn_bwd_dkdv=3, attn_bwd_dq=4,
 NKID = 11
 
 _lib = None
+# the current stream's handle without building a torch.cuda.Stream (1.9 us of a 4 us launch)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def load():
@@ -128,10 +134,11 @@ def call(name, *args):
 
 def call_on(device, name, *args):
     """call(name, *args, stream) on `device`'s current stream, whichever device is current."""
-    if torch.cuda.current_device() == device.index:
-        return call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if torch.cuda.current_device() == index:
+        return call(name, *args, _raw_stream(index))
     with torch.cuda.device(device):
-        return call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+        return call(name, *args, _raw_stream(index))
 
 
 def stream_ptr(device=None):

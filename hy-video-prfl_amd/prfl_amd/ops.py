@@ -425,11 +425,13 @@ def _type(t, what):
     return TYPES[t]
 
 
-def _one_device(what, *tensors):
-    _lib.require_gpu(*tensors)
-    dev = tensors[0].device
-    for t in tensors:
+def _one_device(what, first, *others):
+    if not first.is_cuda:
+        _lib.require_gpu(first)
+    dev = first.device
+    for t in others:
         if t is not None and t.device != dev:
+            _lib.require_gpu(t)
             raise ValueError(f"{what}: tensors on {dev} and {t.device}")
     return dev
 
@@ -461,7 +463,7 @@ def layer_norm_fwd(x, w=None, b=None, eps=1e-5, out_dtype=None):
     L = x2.shape[0]
     y = torch.empty(x.shape, dtype=ydt, device=dev)
     mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
-    rstd = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    rstd = torch.empty_like(mean)
     _lib.call_on(dev, "prfl_layer_norm_fwd", x2.data_ptr(), xt, x2.stride(0), L, C, _addr(w),
                  _addr(b), wt, eps, y.data_ptr(), yt, C, mean.data_ptr(), rstd.data_ptr())
     return y, mean, rstd
@@ -489,14 +491,13 @@ def layer_norm_bwd(dy, x, mean, rstd, w=None, want_dx=True, want_dw=None, want_d
     L = x2.shape[0]
     mean, rstd = mean.contiguous(), rstd.contiguous()
     w = None if w is None else w.contiguous()
-    f32 = dict(dtype=torch.float32, device=dev)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if want_dx else None
-    dw = torch.empty(C, **f32) if want_dw else None
-    db = torch.empty(C, **f32) if want_db else None
+    dx = x.new_empty(x.shape) if want_dx else None
+    dw = mean.new_empty(C) if want_dw else None
+    db = mean.new_empty(C) if want_db else None
     part = None
     if want_dw or want_db:
         n = _lib.load().prfl_layer_norm_parts(L, C, xt)
-        part = torch.empty(max(1, n * C * (int(want_dw) + int(want_db))), **f32)
+        part = mean.new_empty(max(1, n * C * (int(want_dw) + int(want_db))))
     _lib.call_on(dev, "prfl_layer_norm_bwd", dy2.data_ptr(), yt, dy2.stride(0), x2.data_ptr(), xt,
                  x2.stride(0), mean.data_ptr(), rstd.data_ptr(), L, C, _addr(w), wt, _addr(dx), C,
                  _addr(dw), _addr(db), _addr(part))
@@ -642,14 +643,14 @@ def linear_mxfp4(x, wq, ws, out_features, bias=None):
     _mx_check("linear_mxfp4", wq, ws, N, K)
     if bias is not None and (bias.dtype != BF16 or bias.shape != (N,) or not bias.is_contiguous()):
         raise ValueError(f"linear_mxfp4: a contiguous bf16 bias of [{N}]")
-    _type(x.dtype, "linear_mxfp4")
+    xt = _type(x.dtype, "linear_mxfp4")
     x2 = _rows(x, K)
     M = x2.shape[0]
-    y = torch.empty(*x.shape[:-1], N, dtype=BF16, device=dev)
-    if M:
-        xq, xs = quant_mxfp4(x2)
-        _lib.call_on(dev, "prfl_gemm_mxfp4", xq.data_ptr(), xs.data_ptr(), wq.data_ptr(),
-                     ws.data_ptr(), _addr(bias), y.data_ptr(), N, M, N, K)
+    y = torch.empty((*x.shape[:-1], N), dtype=BF16, device=dev)
+    nb = _lib.load().prfl_linear_mxfp4_ws_bytes(M, K)
+    work = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    _lib.call_on(dev, "prfl_linear_mxfp4", x2.data_ptr(), xt, x2.stride(0), wq.data_ptr(),
+                 ws.data_ptr(), _addr(bias), y.data_ptr(), N, M, N, K, _addr(work), nb)
     return y
 
 

@@ -326,6 +326,13 @@ int prfl_dequant_mxfp4(const void* q, const void* s, int64_t M, int64_t K, void*
  * the block-scaled MFMA, fp32 sums, one rounding. */
 int prfl_gemm_mxfp4(const void* xq, const void* xs, const void* wq, const void* ws, const void* bias,
                     void* y, int64_t ldy, int64_t M, int64_t N, int64_t K, void* stream);
+/* The same from x [M][K] as it is (x_type as above, row stride ldx), quantised in the call into `work`
+ * (16-B aligned, prfl_linear_mxfp4_ws_bytes(M, K) bytes; 0 for few rows, which quantise in the
+ * product's own launch). */
+int64_t prfl_linear_mxfp4_ws_bytes(int64_t M, int64_t K);
+int prfl_linear_mxfp4(const void* x, int x_type, int64_t ldx, const void* wq, const void* ws,
+                      const void* bias, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K,
+                      void* work, int64_t work_bytes, void* stream);
 
 /* ---- FlowUniPC sampler update (bh2, order <= 2, x0-prediction) ----------------------------
  * Replaces the element-wise body of FlowUniPCMultistepScheduler.step

@@ -173,7 +173,8 @@ def matrices(M, N, K, seed=0):
                                    (33, 320, 513), (64, 64, 128), (65, 129, 257), (127, 255, 1000),
                                    (128, 128, 256), (129, 300, 640), (255, 511, 896), (256, 256, 1024),
                                    (257, 513, 1152), (300, 1280, 2048), (512, 768, 640),
-                                   (1000, 1000, 1000), (2049, 520, 320)])
+                                   (1000, 1000, 1000), (2049, 520, 320), (5300, 5376, 128),
+                                   (6000, 5000, 200), (9, 200, 14000), (1, 100, 33000), (33, 64, 9000)])
 def test_linear(ops, M, N, K):
     x, w, b = matrices(M, N, K)
     check_linear(ops, x.to(BF16), w, b)
@@ -194,7 +195,8 @@ def exact_matrices(M, N, K, seed=0):
 
 
 @pytest.mark.parametrize("M,N,K", [(1, 160, 5120), (3, 512, 1024), (17, 96, 640), (40, 130, 2048),
-                                   (130, 258, 4096), (300, 200, 5120), (512, 512, 128), (770, 1030, 1152)])
+                                   (130, 258, 4096), (300, 200, 5120), (512, 512, 128), (770, 1030, 1152),
+                                   (6, 320, 5120), (64, 320, 2200), (5500, 5632, 640), (5500, 5600, 384)])
 def test_linear_to_the_bit(ops, M, N, K):
     x, w = exact_matrices(M, N, K)
     y = ops.linear_mxfp4(x.to(BF16), *ops.quant_mxfp4(w), N)

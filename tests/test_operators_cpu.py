@@ -179,6 +179,15 @@ def test_c_entries_refuse(ops):
                 dict(K=0)):
         assert mm(**bad) == 1, bad
     assert mm(M=0) == 0
+    lin = lambda x=p, t=0, ld=32, wq=p, ws=p, y=p, ldy=8, M=2, N=8, K=32, w=None, nb=0: lib.prfl_linear_mxfp4(  # noqa: E731
+        x, t, ld, wq, ws, None, y, ldy, M, N, K, w, nb, None)
+    assert lib.prfl_linear_mxfp4_ws_bytes(2, 32) == 0
+    assert lib.prfl_linear_mxfp4_ws_bytes(65, 129) == 2 * 2 * 4352
+    for bad in (dict(x=None), dict(t=3), dict(t=-1), dict(wq=p + 8), dict(ws=p + 1), dict(y=None), dict(ldy=7),
+                dict(N=0), dict(M=-1), dict(K=0), dict(ld=-1), dict(M=65, K=129),
+                dict(M=65, K=129, w=p, nb=2 * 2 * 4352 - 1), dict(M=65, K=129, w=p + 8, nb=2 * 2 * 4352)):
+        assert lin(**bad) == 1, bad
+    assert lin(M=0) == 0
 
     n, t = (ctypes.c_int64 * 2)(4, 5), (ctypes.c_int32 * 2)(0, 1)
     at, none = (ctypes.c_void_p * 2)(p, p), (ctypes.c_void_p * 2)(p, None)
