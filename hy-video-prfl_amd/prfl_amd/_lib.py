@@ -83,7 +83,7 @@ SIGNATURES = {
     "prfl_layer_norm_parts": [I64, I64, I32],
     "prfl_grads_parts": [P, I64],
     "prfl_grads_sumsq": [P, P, P, I64, P, I64, P, P],
-    "prfl_grads_clip": [P, P, P, P, I64, I32, P, F32, F32, P, P],
+    "prfl_grads_clip": [P, P, P, P, I64, I32, P, P, I64, F32, F32, P, P],
     "prfl_quant_mxfp4": [P, I32, I64, I64, I64, P, P, P],
     "prfl_dequant_mxfp4": [P, P, I64, I64, P, I32, I64, P],
     "prfl_linear_mxfp4_ws_bytes": [I64, I64],

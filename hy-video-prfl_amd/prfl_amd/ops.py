@@ -519,42 +519,44 @@ def _dense(t):
 
 
 def _grad_list(grads, what, disjoint):
-    grads = list(grads)
+    """(addresses, sizes, type codes) of the tensors as host arrays"""
     if not grads:
         raise ValueError(f"{what}: no tensors")
-    _lib.require_gpu(*grads)
+    dev = grads[0].device
+    at, n, types = [], [], []
     for t in grads:
-        if t.layout != torch.strided or t.dtype not in TYPES or not _dense(t):
+        code = TYPES.get(t.dtype)
+        if code is None or t.layout is not torch.strided or not (t.is_contiguous() or _dense(t)):
             raise ValueError(f"{what}: dense fp32, bf16 or fp16 tensors, got {t.dtype} "
-                             f"{tuple(t.shape)} with strides {t.stride() if t.layout == torch.strided else t.layout}")
-        if t.device != grads[0].device:
-            raise ValueError(f"{what}: tensors on {grads[0].device} and {t.device}")
-    n = [t.numel() for t in grads]
-    at = [t.data_ptr() for t in grads]
+                             f"{tuple(t.shape)}, {t.layout}")
+        if t.device != dev:
+            raise ValueError(f"{what}: tensors on {dev} and {t.device}")
+        at.append(t.data_ptr())
+        n.append(t.numel())
+        types.append(code)
     if disjoint:
         end = 0
-        for a, b in sorted((p, p + k * t.element_size()) for p, k, t in zip(at, n, grads) if k):
-            if a < end:
-                raise ValueError(f"{what}: two of the tensors share memory")
-            end = b
+        for a, k, code in sorted(zip(at, n, types)):
+            if k:
+                if a < end:
+                    raise ValueError(f"{what}: two of the tensors share memory")
+                end = a + k * (2 if code else 4)
     k = len(grads)
-    return (grads, (ctypes.c_void_p * k)(*at), (ctypes.c_int64 * k)(*n),
-            (ctypes.c_int32 * k)(*[TYPES[t.dtype] for t in grads]))
-
-
-def _sumsq(grads, at, n, types):
-    dev = grads[0].device
-    parts = _lib.load().prfl_grads_parts(n, len(grads))
-    ws = torch.empty(parts + 1, dtype=torch.float64, device=dev)
-    _lib.call_on(dev, "prfl_grads_sumsq", at, n, types, len(grads), ws.data_ptr(), parts,
-                 ws.data_ptr() + 8 * parts)
-    return ws[parts:]
+    return (ctypes.c_void_p * k)(*at), (ctypes.c_int64 * k)(*n), (ctypes.c_int32 * k)(*types)
 
 
 def grads_sumsq(grads):
     """Sum of the squares of all elements of a list of dense fp32 / bf16 / fp16 tensors: fp64 [1] on
     their device.  (Ranks that hold shards add theirs, then clip_grads(sumsq=...).)"""
-    return _sumsq(*_grad_list(grads, "grads_sumsq", False))
+    grads = list(grads)
+    _lib.require_gpu(*grads)
+    at, n, types = _grad_list(grads, "grads_sumsq", False)
+    dev, k = grads[0].device, len(grads)
+    parts = _lib.load().prfl_grads_parts(n, k)
+    part = torch.empty(parts, dtype=torch.float64, device=dev)
+    out = torch.empty(1, dtype=torch.float64, device=dev)
+    _lib.call_on(dev, "prfl_grads_sumsq", at, n, types, k, part.data_ptr(), parts, out.data_ptr())
+    return out
 
 
 def clip_grads(grads, max_norm, eps=1e-6, out=None, sumsq=None):
@@ -564,27 +566,28 @@ def clip_grads(grads, max_norm, eps=1e-6, out=None, sumsq=None):
     if not max_norm >= 0 or not eps >= 0:
         raise ValueError(f"clip_grads: max_norm and eps are not negative, got {max_norm}, {eps}")
     grads = list(grads)
-    dst, otype = None, -1
-    if out is not None:
-        out = list(out)
-        if len(out) != len(grads) or any(o.shape != g.shape or o.stride() != g.stride()
-                                         or o.dtype != out[0].dtype for o, g in zip(out, grads)):
-            raise ValueError("clip_grads: out has the gradients' shapes and strides, and one type")
-        both, at, n, types = _grad_list(grads + out, "clip_grads", True)
-        k = len(grads)
-        otype = TYPES[out[0].dtype]
-        dst = (ctypes.c_void_p * k)(*at[k:])
-        lists = (grads, at, n, types)       # the first k of each
+    _lib.require_gpu(*grads)
+    dst, otype, k = None, -1, len(grads)
+    if out is None:
+        at, n, types = _grad_list(grads, "clip_grads", True)
     else:
-        lists = _grad_list(grads, "clip_grads", True)
+        out = list(out)
+        if len(out) != k or any(o.shape != g.shape or o.stride() != g.stride()
+                                or o.dtype != out[0].dtype for o, g in zip(out, grads)):
+            raise ValueError("clip_grads: out has the gradients' shapes and strides, and one type")
+        _lib.require_gpu(*out)
+        at, n, types = _grad_list(grads + out, "clip_grads", True)      # first k: the gradients
+        dst, otype = (ctypes.c_void_p * k)(*at[k:]), types[k]
     dev = grads[0].device
+    part, parts = None, 0
     if sumsq is None:
-        sumsq = _sumsq(*lists)
+        parts = _lib.load().prfl_grads_parts(n, k)
+        part = torch.empty(parts, dtype=torch.float64, device=dev)
     elif sumsq.dtype != torch.float64 or sumsq.numel() != 1 or sumsq.device != dev:
         raise ValueError("clip_grads: sumsq is one fp64 value on the gradients' device")
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    _lib.call_on(dev, "prfl_grads_clip", lists[1], dst, lists[2], lists[3], len(grads), otype,
-                 sumsq.data_ptr(), max_norm, eps, norm.data_ptr())
+    _lib.call_on(dev, "prfl_grads_clip", at, dst, n, types, k, otype, _addr(sumsq), _addr(part), parts,
+                 max_norm, eps, norm.data_ptr())
     return norm
 
 

@@ -302,12 +302,14 @@ int64_t prfl_layer_norm_parts(int64_t rows, int64_t C, int x_type);
 int64_t prfl_grads_parts(const int64_t* n, int64_t count);
 int prfl_grads_sumsq(const void* const* grads, const int64_t* n, const int32_t* type, int64_t count,
                      double* part, int64_t parts, double* sumsq, void* stream);
-/* g *= min(1, max_norm / (norm + eps)), norm = sqrt(sumsq[0]); norm[0] (fp32, may be NULL) gets it.
- * out == NULL: in place (nothing is touched when the factor is 1), else out[i] (out_type, as many
- * elements) = the clipped gradient.  A NaN norm makes every gradient NaN. */
+/* g *= min(1, max_norm / (norm + eps)), norm = sqrt(sumsq[0]), or with sumsq == NULL the norm of
+ * these tensors (part / parts as above); norm[0] (fp32, may be NULL) gets it.  out == NULL (out_type
+ * -1): in place (nothing is touched when the factor is 1), else out[i] (out_type, as many elements) =
+ * the clipped gradient.  A NaN norm makes every gradient NaN. */
 int prfl_grads_clip(const void* const* grads, void* const* out, const int64_t* n,
                     const int32_t* type, int64_t count, int out_type, const double* sumsq,
-                    float max_norm, float eps, float* norm, void* stream);
+                    double* part, int64_t parts, float max_norm, float eps, float* norm,
+                    void* stream);
 
 /* ---- microscaled fp4 (OCP MX: e2m1 elements, one e8m0 scale per 32 of a row) ------------------
  * Beside the e4m3 path: nn.Linear forwards of a frozen trunk (the latent reward model,

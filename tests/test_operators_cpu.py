@@ -196,8 +196,9 @@ def test_c_entries_refuse(ops):
     for bad in (dict(at=none), dict(parts=1), dict(c=-1), dict(s=None), dict(t=(ctypes.c_int32 * 2)(0, 3)),
                 dict(n=(ctypes.c_int64 * 2)(4, -1))):
         assert ss(**bad) == 1, bad
-    cl = lambda at=at, out=None, c=2, ot=-1, s=p, m=1.0, e=1e-6: lib.prfl_grads_clip(  # noqa: E731
-        at, out, n, t, c, ot, s, m, e, p, None)
-    for bad in (dict(at=none), dict(out=none, ot=0), dict(ot=0), dict(ot=3), dict(s=None), dict(m=-1.0),
-                dict(m=float("nan")), dict(e=-1.0), dict(c=-1)):
+    cl = lambda at=at, out=None, c=2, ot=-1, s=p, w=None, parts=0, m=1.0, e=1e-6: lib.prfl_grads_clip(  # noqa: E731
+        at, out, n, t, c, ot, s, w, parts, m, e, p, None)
+    for bad in (dict(at=none), dict(out=none, ot=0), dict(ot=0), dict(out=at), dict(out=at, ot=3), dict(m=-1.0),
+                dict(m=float("nan")), dict(e=-1.0), dict(c=-1), dict(s=None), dict(s=None, w=p, parts=1),
+                dict(s=None, parts=2)):
         assert cl(**bad) == 1, bad
