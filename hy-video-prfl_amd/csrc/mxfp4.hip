@@ -317,6 +317,14 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void mx_rows_kernel(MxArgs a, cons
 // RAW: step j+1 is read after the barrier that every wave passes with its part of it landed.  WAR: the
 // slot of step j-1 was read for MFMAs that precede this barrier in every wave.  Past the last
 // step the DMA fetches it again into a slot nobody reads, so the count is the same every step.
+//
+// WT 4: 32760 x 13824 x 5120 takes 1.16 ms = 4.0 PFLOP/s.  MFMAs alone on random operands run at 6.0 to 6.6 PFLOP/s (the
+// clock falls to 1.5 GHz); here they are busy 54 % of 1.74 GHz, beside 96 B a clock of LDS traffic of a
+// possible 128.  Measured and dropped: one workgroup per CU walking its tiles as one stream of steps, the
+// finished tile held in registers and stored during the next one's steps: 1.16 ms too.
+// WT 2: LDS sets the time, 48 KiB a step per CU against 256 cycles of MFMAs (512 x 5120 x 4096: 12 us, of which 5 us are
+// launch, first loads and stores).  Measured and dropped, no faster: an eight-slot ring, fragments read a whole
+// step ahead, and two groups of waves that share K.
 template <int WT>
 __global__ __launch_bounds__(NT, WT == 4 ? 1 : 2) void mx_gemm_tile_kernel(MxArgs a) {
   constexpr int OPB = WT * PIECE, OPS = WT * PIECE_S, SLOT = 2 * (OPB + OPS);
@@ -440,9 +448,10 @@ __global__ __launch_bounds__(NT, WT == 4 ? 1 : 2) void mx_gemm_tile_kernel(MxArg
 
   const int n0 = tn * 64 * WT + wn * 32 * WT;
   const int64_t m0 = (int64_t)tm * 64 * WT + wm * 32 * WT;
-  // A tile whose columns are all there, with 16-B aligned rows, leaves through a wave-private LDS image (32 rows of the wave's
-  // columns at a time, 16 B of padding a row), so that a store instruction writes whole cache lines; in the
-  // MFMA layout it would write 64 pieces of 8 B.
+  // A tile whose columns are all there, with 16-B aligned rows, leaves through a wave-private LDS image (16 B of
+  // padding a row), so that a store instruction writes whole lines; in the MFMA layout it would write 64
+  // pieces of 8 B (32760 x 13824 x 5120: 1.77 ms so, 1.16 ms through the image).  Non-temporal, past the operands in
+  // L2 (1.20 ms without).
   constexpr int RB = 64 * WT, ROW = RB + 16, LPR = RB / 16, RPI = 64 / LPR;
   static_assert(4 * WT * 32 * ROW <= 4 * SLOT, "the images reuse the ring");
   if ((tn + 1) * 64 * WT <= a.N && a.ldy % 8 == 0 && ((uintptr_t)a.y & 15) == 0) {
@@ -473,7 +482,8 @@ __global__ __launch_bounds__(NT, WT == 4 ? 1 : 2) void mx_gemm_tile_kernel(MxArg
 #pragma unroll
     for (int t = 0; t < WT * 32 / RPI; ++t)
       if (m0 + t * RPI + lane / LPR < a.M)
-        *(u32x4*)(y0 + (int64_t)t * RPI * a.ldy) = *(const u32x4*)(img + (t * RPI + lane / LPR) * ROW + (lane % LPR) * 16);
+        __builtin_nontemporal_store(*(const u32x4*)(img + (t * RPI + lane / LPR) * ROW + (lane % LPR) * 16),
+                                    (u32x4*)(y0 + (int64_t)t * RPI * a.ldy));
     return;
   }
 #pragma unroll
