@@ -461,8 +461,9 @@ def layer_norm_fwd(x, w=None, b=None, eps=1e-5, out_dtype=None):
     w, b = (v if v is None else v.contiguous() for v in (w, b))
     x2 = _rows(x, C)
     L = x2.shape[0]
-    y = torch.empty(x.shape, dtype=ydt, device=dev)
-    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    # (new_empty and empty_like cost half of torch.empty(device=) on the host, a third of a short call)
+    y = torch.empty_like(x, dtype=ydt) if x.is_contiguous() else x.new_empty(x.shape, dtype=ydt)
+    mean = x.new_empty(L if x.dim() == 2 else x.shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
     _lib.call_on(dev, "prfl_layer_norm_fwd", x2.data_ptr(), xt, x2.stride(0), L, C, _addr(w),
                  _addr(b), wt, eps, y.data_ptr(), yt, C, mean.data_ptr(), rstd.data_ptr())
@@ -491,7 +492,9 @@ def layer_norm_bwd(dy, x, mean, rstd, w=None, want_dx=True, want_dw=None, want_d
     L = x2.shape[0]
     mean, rstd = mean.contiguous(), rstd.contiguous()
     w = None if w is None else w.contiguous()
-    dx = x.new_empty(x.shape) if want_dx else None
+    dx = None
+    if want_dx:
+        dx = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
     dw = mean.new_empty(C) if want_dw else None
     db = mean.new_empty(C) if want_db else None
     part = None
@@ -522,6 +525,7 @@ def _grad_list(grads, what, disjoint):
     """(addresses, sizes, type codes) of the tensors as host arrays"""
     if not grads:
         raise ValueError(f"{what}: no tensors")
+    _lib.require_gpu(grads[0])
     dev = grads[0].device
     at, n, types = [], [], []
     for t in grads:
@@ -549,7 +553,6 @@ def grads_sumsq(grads):
     """Sum of the squares of all elements of a list of dense fp32 / bf16 / fp16 tensors: fp64 [1] on
     their device.  (Ranks that hold shards add theirs, then clip_grads(sumsq=...).)"""
     grads = list(grads)
-    _lib.require_gpu(*grads)
     at, n, types = _grad_list(grads, "grads_sumsq", False)
     dev, k = grads[0].device, len(grads)
     parts = _lib.load().prfl_grads_parts(n, k)
@@ -566,7 +569,6 @@ def clip_grads(grads, max_norm, eps=1e-6, out=None, sumsq=None):
     if not max_norm >= 0 or not eps >= 0:
         raise ValueError(f"clip_grads: max_norm and eps are not negative, got {max_norm}, {eps}")
     grads = list(grads)
-    _lib.require_gpu(*grads)
     dst, otype, k = None, -1, len(grads)
     if out is None:
         at, n, types = _grad_list(grads, "clip_grads", True)
@@ -575,7 +577,6 @@ def clip_grads(grads, max_norm, eps=1e-6, out=None, sumsq=None):
         if len(out) != k or any(o.shape != g.shape or o.stride() != g.stride()
                                 or o.dtype != out[0].dtype for o, g in zip(out, grads)):
             raise ValueError("clip_grads: out has the gradients' shapes and strides, and one type")
-        _lib.require_gpu(*out)
         at, n, types = _grad_list(grads + out, "clip_grads", True)      # first k: the gradients
         dst, otype = (ctypes.c_void_p * k)(*at[k:]), types[k]
     dev = grads[0].device
@@ -606,8 +607,8 @@ def quant_mxfp4(x):
     M, K = x.shape
     x = _rows(x, K)
     G, S = _mx_shape(M, K)
-    q = torch.empty(G, S, 4, 64, 16, dtype=torch.uint8, device=dev)
-    s = torch.empty(G, S, 64, 4, dtype=torch.uint8, device=dev)
+    q = x.new_empty((G, S, 4, 64, 16), dtype=torch.uint8)
+    s = q.new_empty((G, S, 64, 4))
     _lib.call_on(dev, "prfl_quant_mxfp4", x.data_ptr(), xt, x.stride(0), M, K, q.data_ptr(),
                  s.data_ptr())
     return q, s
@@ -630,7 +631,7 @@ def dequant_mxfp4(q, s, rows, cols, out_dtype=BF16):
     _mx_check("dequant_mxfp4", q, s, rows, cols)
     if out_dtype not in (BF16, torch.float32):
         raise ValueError(f"dequant_mxfp4: bf16 or fp32, got {out_dtype}")
-    out = torch.empty(rows, cols, dtype=out_dtype, device=dev)
+    out = q.new_empty((rows, cols), dtype=out_dtype)
     _lib.call_on(dev, "prfl_dequant_mxfp4", q.data_ptr(), s.data_ptr(), rows, cols, out.data_ptr(),
                  int(out_dtype == torch.float32), cols)
     return out
@@ -649,9 +650,9 @@ def linear_mxfp4(x, wq, ws, out_features, bias=None):
     xt = _type(x.dtype, "linear_mxfp4")
     x2 = _rows(x, K)
     M = x2.shape[0]
-    y = torch.empty((*x.shape[:-1], N), dtype=BF16, device=dev)
+    y = x.new_empty((*x.shape[:-1], N), dtype=BF16)
     nb = _lib.load().prfl_linear_mxfp4_ws_bytes(M, K)
-    work = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    work = wq.new_empty(nb) if nb else None
     _lib.call_on(dev, "prfl_linear_mxfp4", x2.data_ptr(), xt, x2.stride(0), wq.data_ptr(),
                  ws.data_ptr(), _addr(bias), y.data_ptr(), N, M, N, K, _addr(work), nb)
     return y
