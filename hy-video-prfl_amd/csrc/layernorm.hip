@@ -347,7 +347,14 @@ int grid_for_rows(int64_t rows, const Split& s, int waves) {
   return (int)(g < most ? g : most);
 }
 constexpr int FWD_WAVES = 16, FWD_NARROW_WAVES = 24, BWD_WAVES = 12;
-int bwd_grid(int64_t rows, const Split& s) { return rows ? grid_for_rows(rows, s, BWD_WAVES) : 0; }
+// The backward's workgroups each leave C partial sums: 256 of them (one a CU), and more where each still has
+// four turns (1003 x 1021 fp16: 13 us in 256 workgroups, 18 in 1003).
+int bwd_grid(int64_t rows, const Split& s) {
+  if (!rows) return 0;
+  const int g = grid_for_rows(rows, s, BWD_WAVES);
+  const int64_t turns = (rows + 4 * s.rows_at_once() - 1) / (4 * s.rows_at_once());
+  return g <= 256 || turns >= g ? g : (int)(turns > 256 ? turns : 256);
+}
 
 template <typename F>
 void by_types(int xt, int yt, F f) {               // f(null pointers of the two types)
