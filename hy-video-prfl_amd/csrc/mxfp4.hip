@@ -151,21 +151,7 @@ struct MxArgs {
 };
 
 // W is the MFMA's first operand, so a lane holds four consecutive columns n of one row m at a
-// time: register r of tile (i, j) is n = 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4, m = 32 j + lane % 32
-__device__ __forceinline__ void store4(const MxArgs& a, int64_t m, int n, const float (&v)[4]) {
-  if (m >= a.M) return;
-  bf16* p = a.y + m * a.ldy + n;
-  if (n + 4 <= a.N) {
-    typename Loaded<bf16, 4>::vec t;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t[i] = f2bf(v[i] + (a.bias ? bf2f(a.bias[n + i]) : 0.f));
-    *(typename Loaded<bf16, 4>::at*)p = t;
-  } else {
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < a.N) p[i] = f2bf(v[i] + (a.bias ? bf2f(a.bias[n + i]) : 0.f));
-  }
-}
+// time: register 4 q + c of a 32 x 32 tile is n = 8 q + 4 (lane / 32) + c, m = lane % 32
 
 // tile of workgroup bid: every eighth workgroup runs on the same XCD, so XCD k gets the k-th eighth of
 // the tiles, and within it 8 tile rows advance over the tile columns together (their operands
@@ -448,53 +434,61 @@ __global__ __launch_bounds__(NT, WT == 4 ? 1 : 2) void mx_gemm_tile_kernel(MxArg
 
   const int n0 = tn * 64 * WT + wn * 32 * WT;
   const int64_t m0 = (int64_t)tm * 64 * WT + wm * 32 * WT;
-  // A tile whose columns are all there, with 16-B aligned rows, leaves through a wave-private LDS image (16 B of
-  // padding a row), so that a store instruction writes whole lines; in the MFMA layout it would write 64
-  // pieces of 8 B (32760 x 13824 x 5120: 1.77 ms so, 1.16 ms through the image).  Non-temporal, past the operands in
-  // L2 (1.20 ms without).
-  constexpr int RB = 64 * WT, ROW = RB + 16, LPR = RB / 16, RPI = 64 / LPR;
+  // The tile leaves through a wave-private LDS image (16 B of padding a row), so that a store instruction writes
+  // whole lines; in the MFMA layout it would write 64 pieces of 8 B (32760 x 13824 x 5120: 1.77 ms so, 1.16 ms
+  // through the image).  Non-temporal, past the operands in L2 (1.20 ms without).  Rows need not be aligned.
+  constexpr int ROW = 64 * WT + 16, LPR = 4 * WT, RPI = 64 / LPR;
   static_assert(4 * WT * 32 * ROW <= 4 * SLOT, "the images reuse the ring");
-  if ((tn + 1) * 64 * WT <= a.N && a.ldy % 8 == 0 && ((uintptr_t)a.y & 15) == 0) {
-    typename Loaded<bf16, 4>::vec b[WT][4];
+  bf16x4 b[WT][4];
+  if (a.bias && (tn + 1) * 64 * WT <= a.N) {
+#pragma unroll
+    for (int i = 0; i < WT * 4; ++i)
+      b[i >> 2][i & 3] = *(const typename Loaded<bf16, 4>::at*)(a.bias + n0 + i * 8 + 4 * (lane >> 5));
+  } else {
+#pragma unroll
+    for (int i = 0; i < WT * 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int n = n0 + i * 8 + 4 * (lane >> 5) + k;
+        b[i >> 2][i & 3][k] = a.bias && n < a.N ? a.bias[n] : (bf16)0.f;
+      }
+  }
+  __builtin_amdgcn_s_barrier();            // every wave's DMA has landed and its fragments are read
+  asm volatile("" ::: "memory");
+  char* img = smem + wid * (WT * 32 * ROW);
+#pragma unroll
+  for (int jj = 0; jj < WT; ++jj)
 #pragma unroll
     for (int i = 0; i < WT; ++i)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        b[i][r] = (typename Loaded<bf16, 4>::vec){};
-        if (a.bias) b[i][r] = *(const typename Loaded<bf16, 4>::at*)(a.bias + n0 + i * 32 + 8 * r + 4 * (lane >> 5));
+        bf16x4 o;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = f2bf(acc[i][jj][4 * r + k] + bf2f(b[i][r][k]));
+        *(bf16x4*)(img + (jj * 32 + (lane & 31)) * ROW + (i * 32 + 8 * r + 4 * (lane >> 5)) * 2) = o;
       }
-    __builtin_amdgcn_s_barrier();          // every wave's DMA has landed and its fragments are read
-    asm volatile("" ::: "memory");
-    char* img = smem + wid * (WT * 32 * ROW);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  const int n = n0 + (lane % LPR) * 8;
+  bf16* const y0 = a.y + (m0 + lane / LPR) * a.ldy + n;
+  const bool inside = (tn + 1) * 64 * WT <= a.N && (int64_t)(tm + 1) * 64 * WT <= a.M;
 #pragma unroll
-    for (int jj = 0; jj < WT; ++jj)
+  for (int t0 = 0; t0 < WT * 32 / RPI; t0 += 8) {
+    bf16x8 o[8];
 #pragma unroll
-      for (int i = 0; i < WT; ++i)
+    for (int t = 0; t < 8; ++t)
+      o[t] = *(const bf16x8*)(img + ((t0 + t) * RPI + lane / LPR) * ROW + (lane % LPR) * 16);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          bf16x4 o;
+    for (int t = 0; t < 8; ++t) {
+      bf16* p = y0 + (int64_t)(t0 + t) * RPI * a.ldy;
+      if (inside || (m0 + (t0 + t) * RPI + lane / LPR < a.M && n + 8 <= a.N)) {
+        __builtin_nontemporal_store(o[t], (typename Loaded<bf16, 8>::at*)p);
+      } else if (m0 + (t0 + t) * RPI + lane / LPR < a.M) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) o[k] = f2bf(acc[i][jj][4 * r + k] + bf2f(b[i][r][k]));
-          *(bf16x4*)(img + (jj * 32 + (lane & 31)) * ROW + (i * 32 + 8 * r + 4 * (lane >> 5)) * 2) = o;
-        }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    bf16* const y0 = a.y + (m0 + lane / LPR) * a.ldy + n0 + (lane % LPR) * 8;
-#pragma unroll
-    for (int t = 0; t < WT * 32 / RPI; ++t)
-      if (m0 + t * RPI + lane / LPR < a.M)
-        __builtin_nontemporal_store(*(const u32x4*)(img + (t * RPI + lane / LPR) * ROW + (lane % LPR) * 16),
-                                    (u32x4*)(y0 + (int64_t)t * RPI * a.ldy));
-    return;
+        for (int k = 0; k < 8; ++k)
+          if (n + k < a.N) p[k] = o[t][k];
+      }
+    }
   }
-#pragma unroll
-  for (int i = 0; i < WT; ++i)
-#pragma unroll
-    for (int jj = 0; jj < WT; ++jj)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float v[4] = {acc[i][jj][4 * r], acc[i][jj][4 * r + 1], acc[i][jj][4 * r + 2], acc[i][jj][4 * r + 3]};
-        store4(a, m0 + jj * 32 + (lane & 31), n0 + i * 32 + 8 * r + 4 * (lane >> 5), v);
-      }
 }
 
 constexpr int ROWS_MOST = 64;

@@ -515,7 +515,11 @@ def linear_mxfp4_backward(dy: Tensor, wq: Tensor, ws: Tensor, in_features: int, 
         d = dy.reshape(-1, N).to(BF16)
         if N % 8:
             d = torch.nn.functional.pad(d, (0, -N % 8))
-        db = ops.colsum(d.contiguous())[:N].contiguous()
+        if d.shape[0]:
+            with torch.cuda.device(d.device):
+                db = ops.colsum(d.contiguous())[:N].contiguous()
+        else:
+            db = torch.zeros(N, dtype=F32, device=d.device)
     return dx, db
 
 

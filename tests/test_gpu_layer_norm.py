@@ -171,6 +171,11 @@ def test_empty(ops):
     assert y.shape == dx.shape == x.shape and not dw.any() and not db.any()
 
 
+def test_one_axis(ops):
+    x, w, b, dy = inputs((1, 300), BF16)
+    check(ops, x[0], w, b, dy[0])
+
+
 def test_wanted_outputs_only(ops):
     x, w, b, dy = inputs((70, 300), F32)
     _, mean, rstd = ops.layer_norm_fwd(x, w, b)
@@ -216,6 +221,40 @@ def test_captured_and_replayed(ops):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(want, got)), k
+
+
+def test_two_graphs_replayed_in_turn(ops):
+    """each holds its own workspace: replays in any order, and eager calls between, change nothing"""
+    from prfl_amd import custom_ops
+
+    def build(seed):
+        x, w, b, dy = inputs((700, 384), BF16, seed=seed)
+        leaves = [t.detach().clone().requires_grad_() for t in (x, w, b)]
+        dy = dy.to(BF16)
+
+        def step():
+            y = custom_ops.layer_norm(*leaves, 1e-6)
+            return (y.detach(),) + torch.autograd.grad(y, leaves, dy)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = [t.clone() for t in step()]
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = step()
+        return graph, got, want, (leaves, dy)           # what the graph reads lives as long as it
+    a, b = build(1), build(2)
+    x, w, bb, dy = inputs((900, 640), F32)
+    for order in ((a, b), (b, a), (a, a, b)):
+        for graph, *_ in order:
+            graph.replay()
+        _, m, r = ops.layer_norm_fwd(x, w, bb)
+        ops.layer_norm_bwd(dy, x, m, r, w)
+        torch.cuda.synchronize()
+        for _, got, want, _ in (a, b):
+            assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
 def test_autograd_op(ops):

@@ -280,6 +280,37 @@ def test_captured_replayed_and_on_another_stream(ops):
             assert all(torch.equal(a, c) for a, c in zip(want, got)), (M, k)
 
 
+def test_two_graphs_replayed_in_turn(ops):
+    built = []
+    for M in (300, 40, 3):
+        x, w, b = matrices(M, 384, 640)
+        wq, ws = ops.quant_mxfp4(w)
+        want = ops.linear_mxfp4(x, wq, ws, 384, b)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = ops.linear_mxfp4(x, wq, ws, 384, b)
+        built.append((graph, got, want, (x, wq, ws, b)))
+    for order in ((0, 1, 2), (2, 0, 1, 0), (1, 1, 2)):
+        for i in order:
+            built[i][1].zero_()
+            built[i][0].replay()
+        ops.linear_mxfp4(built[0][3][0] * 2, *built[0][3][1:3], 384)
+        torch.cuda.synchronize()
+        for i in set(order):
+            assert torch.equal(built[i][1], built[i][2])
+
+
+def test_weights_with_a_nan_block(ops):
+    """its own column of y is NaN, and no other"""
+    for M in (2, 50, 200):
+        x, w, b = matrices(M, 150, 200)
+        w[70, 40] = math.nan
+        y = ops.linear_mxfp4(x, *ops.quant_mxfp4(w), 150, b)
+        bad = y.isnan()
+        assert bad[:, 70].all() and int(bad.sum()) == M
+
+
 def test_autograd_op(ops):
     from prfl_amd import custom_ops
     x, w, b = matrices(12, 72, 96)
@@ -294,4 +325,12 @@ def test_autograd_op(ops):
     assert ((db.double() - ref).abs() <= 2.0 ** -8 * ref.abs() + 12 * 2.0 ** -24 * dy.double().abs().view(
         12, 72).sum(0)).all()
     assert torch.autograd.grad(custom_ops.linear_mxfp4(xl, wq, ws, 72, None), xl, dy)[0].shape == xl.shape
+    w2, ws2 = ops.quant_mxfp4(w[:71])                             # a width that the column sums pad
+    b2 = b[:71].clone().requires_grad_()
+    db = torch.autograd.grad(custom_ops.linear_mxfp4(xl, w2, ws2, 71, b2), b2, dy[..., :71])[0]
+    assert ((db.double() - ref[:71]).abs() <= 2.0 ** -8 * ref[:71].abs() + 12 * 2.0 ** -24 * dy.double().abs().view(
+        12, 72).sum(0)[:71]).all()
+    none = custom_ops.linear_mxfp4(xl[:0], wq, ws, 72, bl)
+    dx, db = torch.autograd.grad(none.sum(), (xl, bl))
+    assert not dx.any() and not db.any()
     torch.library.opcheck(torch.ops.prfl.linear_mxfp4, (xl, wq, ws, 72, bl))
