@@ -426,7 +426,7 @@ extern "C" int prfl_layer_norm_bwd(const void* dy, int y_type, int64_t lddy, con
                                    int64_t C, const void* w, int w_type, void* dx, int64_t lddx,
                                    float* dw, float* db, float* part, void* stream) {
   if (bad(rows, C, x_type, y_type, w_type) || (rows > 1 && (ldx < 0 || lddy < 0 || (dx && lddx < C))) ||
-      ((dw || db) && !part))
+      ((dw || db) && !part) || (rows && (dx || dw || db) && (!dy || !x || !mean || !rstd)))
     return (int)hipErrorInvalidValue;
   hipStream_t s = (hipStream_t)stream;
   const Split sp = split_for((int)C, x_type, BWD_WIDE);
@@ -435,7 +435,6 @@ extern "C" int prfl_layer_norm_bwd(const void* dy, int y_type, int64_t lddy, con
   float* pb = db ? part + (dw ? (int64_t)grid * C : 0) : nullptr;
   prfl_prof::begin(KID_LN, s);
   if (rows && (dx || dw || db)) {
-    if (!dy || !x || !mean || !rstd) return (int)hipErrorInvalidValue;
     by_types(x_type, y_type, [&](auto* tx, auto* ty) {
       using TX = std::remove_const_t<std::remove_pointer_t<decltype(tx)>>;
       using TY = std::remove_const_t<std::remove_pointer_t<decltype(ty)>>;

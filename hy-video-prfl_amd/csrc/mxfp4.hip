@@ -1,7 +1,7 @@
 // Microscaled four-bit floating point (OCP MX, e2m1 elements with one e8m0 scale per 32 elements
 // of a row): quantisation, reading back, and the product y = x W^T + b on the block-scaled MFMA.
 //
-//   e    = floor(log2(max |v|)) - 2 over the 32, at least -127   (0 for an all-zero block: -127)
+//   e    = floor(log2(max |v|)) - 2 over the 32, at least -127 (as for a block of zeros)
 //   code = v / 2^e rounded to the nearest of 0 .5 1 1.5 2 3 4 6, ties to the even code, at most 6
 //   a block with a NaN or an infinity has the scale 0xff: all its 32 values read back as NaN.
 //
@@ -16,8 +16,6 @@
 
 namespace {
 typedef __attribute__((ext_vector_type(8))) int i32x8;
-typedef __attribute__((ext_vector_type(2))) _Float16 f16x2;
-typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2;
 
 constexpr int NT = 256;
 constexpr int PIECE = 4096, PIECE_S = 256;        // bytes of a piece: codes, scales
@@ -170,11 +168,13 @@ __device__ __forceinline__ void dma4_step(i32x4 srd, uint32_t voff, uint32_t sof
                :: "v"(voff), "s"(srd), "s"(__builtin_amdgcn_readfirstlane(soff)) : "memory");
 }
 
-// Few rows (M <= 32 MT, MT 1 or 2): 32 columns of y per workgroup, its 16 waves taking every 16th step of
-// 128 along K, their partial sums joined through LDS in wave order.  W is read once, in lane order, with up to
-// four steps of it in flight per wave: the time is W's bytes.  FUSED: x comes as it is, at most 1024 blocks
-// of 32, and every workgroup quantises all of it, a block per thread, into LDS ([block][row]: rows beyond M
-// take no room) -- one launch instead of two, while W's first loads are under way; else x comes tiled.
+// Few rows, or few columns and a long K: 32 MT rows (MT 1 or 2; blockIdx.y) x 32 columns of y per workgroup, its
+// 16 waves taking every 16th step of 128 along K, their partial sums joined through LDS in wave order.  W is
+// read once per row group, in lane order, with up to four steps of it in flight per wave: the time is that of
+// launch, first loads and the join (5120 x 5120, one round of workgroups: 4.5 us for 32 rows, 6.0 for 64).
+// FUSED: x comes as it is, at most 32 rows and 1024 blocks of 32, and every workgroup quantises all of it, a
+// block per thread, into LDS ([block][row]: rows beyond M take no room) -- one launch instead of two, while W's
+// first loads are under way; else x comes tiled.
 template <typename T, int N>
 __device__ __forceinline__ void load_block(const T* p, int n, float (&v)[N]) {
 #pragma unroll
@@ -199,7 +199,9 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void mx_rows_kernel(MxArgs a, cons
   __shared__ uint8_t lsx[FUSED ? ROWS_FUSED : 1];
   const int lane = threadIdx.x & 63, row = lane & 31, blk = lane >> 5;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int nt = blockIdx.x, steps = a.steps, M = (int)a.M;
+  const int nt = blockIdx.x, steps = a.steps;
+  const int64_t g = blockIdx.y;                     // row piece
+  const int M = (int)min(a.M - g * 64, (int64_t)64);
   const uint8_t* w = a.wq + (int64_t)(nt >> 1) * steps * PIECE + (nt & 1) * 2048 + lane * 16;
   const uint8_t* sw = a.ws + (int64_t)(nt >> 1) * steps * PIECE_S + lane * 4;
   constexpr int AHEAD = 4;
@@ -262,10 +264,10 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void mx_rows_kernel(MxArgs a, cons
             }
           }
         } else if (m * 32 + row < M) {
-          const uint8_t* xp = a.xq + (int64_t)k * PIECE + m * 2048 + lane * 16;
+          const uint8_t* xp = a.xq + (g * steps + k) * PIECE + m * 2048 + lane * 16;
           xv[0] = *(const u32x4*)xp;
           xv[1] = *(const u32x4*)(xp + 1024);
-          sx = *(const uint32_t*)(a.xs + (int64_t)k * PIECE_S + lane * 4) >> (16 * m);
+          sx = *(const uint32_t*)(a.xs + (g * steps + k) * PIECE_S + lane * 4) >> (16 * m);
         }
         acc[m] = mfma4<0, 0>(wv[u][0], xv[0], acc[m], sv[u], sx);
         acc[m] = mfma4<1, 1>(wv[u][1], xv[1], acc[m], sv[u], sx);
@@ -288,7 +290,7 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void mx_rows_kernel(MxArgs a, cons
       float s = 0.f;
 #pragma unroll
       for (int i = 0; i < ROWS_WAVES; ++i) s += part[i * 1024 + t];
-      a.y[mm * a.ldy + n] = f2bf(s + (a.bias ? bf2f(a.bias[n]) : 0.f));
+      a.y[(g * 64 + mm) * a.ldy + n] = f2bf(s + (a.bias ? bf2f(a.bias[n]) : 0.f));
     }
   }
 }
@@ -491,21 +493,38 @@ __global__ __launch_bounds__(NT, WT == 4 ? 1 : 2) void mx_gemm_tile_kernel(MxArg
   }
 }
 
-constexpr int ROWS_MOST = 64;
+// Which kernel, by measured kernel times in us (rows / 128 tile, K 5120 where none is named):
+//   mx_rows_kernel while its workgroups come in about one round of the chip (at most 256; up to 384 where K is
+//   long, where a tile's own loop is what takes time; for 32 rows, whose workgroups are half the work, 512):
+//     32 x 5120  4.5 / 11.8    32 x 13824  10.7 / 13.2    64 x 5120 6.0 / 11.8   64 x 10240 11.0 / 12.3   64 x 13824
+//     13.9 / 13.5    192 x 4096 10.5 / 12.0 (K 1280: 7.1 / 6.1)    256 x 1280 6.1 / 11.1    512 x 1280 10.3 / 11.7
+//     128 x 8192 (K 4096) 15.0 / 10.2    300 x 100 (K 14000) 9.4 / 25.8    768 x 1024 (K 13824) 21.0 / 27.5
+//     16 x 65536 (K 4096) 36 / 24
+//   the 256 tile from 432 of them on, nearly two rounds (256 / 128 tile): 4096 x 5120 (320 tiles) 76 / 64,
+//     5000 x 5120 (400) 79 / 81, 2048 x 13824 (432) 81 / 83, 6000 x 5120 (480) 84.5 / 93, 8190 x 5120 (640) 120 / 122,
+//     16000 x 5120 (1260) 213 / 234
+bool by_rows(int64_t M, int64_t N, int steps) {
+  const int64_t n = ((M + 63) / 64) * ((N + 31) / 32);
+  return n <= 256 || (n <= 384 && steps >= 20) || (M <= 32 && n <= 512);
+}
 
 void launch_product(const MxArgs& a, hipStream_t st) {
   const int64_t t256 = ((a.M + 255) / 256) * ((a.N + 255) / 256), t128 = ((a.M + 127) / 128) * ((a.N + 127) / 128);
-  const dim3 cols((unsigned)((a.N + 31) / 32));
-  if (a.M <= 32)
-    hipLaunchKernelGGL((mx_rows_kernel<bf16, 1, false>), cols, dim3(64 * ROWS_WAVES), 0, st, a, nullptr, 0, 0);
-  else if (a.M <= ROWS_MOST)
-    hipLaunchKernelGGL((mx_rows_kernel<bf16, 2, false>), cols, dim3(64 * ROWS_WAVES), 0, st, a, nullptr, 0, 0);
-  else if (t256 >= 432)
+  const dim3 cols((unsigned)((a.N + 31) / 32), (unsigned)((a.M + 63) / 64));
+  if (by_rows(a.M, a.N, a.steps)) {
+    if (a.M <= 32)
+      hipLaunchKernelGGL((mx_rows_kernel<bf16, 1, false>), cols, dim3(64 * ROWS_WAVES), 0, st, a, nullptr, 0, 0);
+    else
+      hipLaunchKernelGGL((mx_rows_kernel<bf16, 2, false>), cols, dim3(64 * ROWS_WAVES), 0, st, a, nullptr, 0, 0);
+  } else if (t256 >= 432) {
     hipLaunchKernelGGL(mx_gemm_tile_kernel<4>, dim3((unsigned)t256), dim3(NT), 0, st, a);
-  else
+  } else {
     hipLaunchKernelGGL(mx_gemm_tile_kernel<2>, dim3((unsigned)t128), dim3(NT), 0, st, a);
+  }
 }
 
+// One launch for both: every workgroup quantises all of x, so only while that is a block a thread (5120 x 5120,
+// one row: 5.2 us against 4.3 + 4.3 in two launches).
 bool fused(int64_t M, int64_t K) { return M <= 32 && M * ((K + 31) / 32) <= ROWS_FUSED; }
 
 bool too_large(int64_t rows, int64_t cols) {       // pieces are counted in 31 bits

@@ -174,7 +174,10 @@ def matrices(M, N, K, seed=0):
                                    (128, 128, 256), (129, 300, 640), (255, 511, 896), (256, 256, 1024),
                                    (257, 513, 1152), (300, 1280, 2048), (512, 768, 640),
                                    (1000, 1000, 1000), (2049, 520, 320), (5300, 5376, 128),
-                                   (6000, 5000, 200), (9, 200, 14000), (1, 100, 33000), (33, 64, 9000)])
+                                   (6000, 5000, 200), (9, 200, 14000), (1, 100, 33000), (33, 64, 9000),
+                                   (65, 6209, 257), (127, 6400, 130), (129, 5119, 640), (257, 2500, 1152),
+                                   (32, 12320, 384), (21, 17000, 96), (300, 100, 14000), (2000, 100, 513),
+                                   (1500, 500, 2600), (1500, 500, 2400), (16385, 20, 40)])
 def test_linear(ops, M, N, K):
     x, w, b = matrices(M, N, K)
     check_linear(ops, x.to(BF16), w, b)
@@ -196,7 +199,8 @@ def exact_matrices(M, N, K, seed=0):
 
 @pytest.mark.parametrize("M,N,K", [(1, 160, 5120), (3, 512, 1024), (17, 96, 640), (40, 130, 2048),
                                    (130, 258, 4096), (300, 200, 5120), (512, 512, 128), (770, 1030, 1152),
-                                   (6, 320, 5120), (64, 320, 2200), (5500, 5632, 640), (5500, 5600, 384)])
+                                   (6, 320, 5120), (64, 320, 2200), (5500, 5632, 640), (5500, 5600, 384),
+                                   (512, 1280, 2688), (384, 2048, 640), (1023, 129, 4100), (12, 16500, 300)])
 def test_linear_to_the_bit(ops, M, N, K):
     x, w = exact_matrices(M, N, K)
     y = ops.linear_mxfp4(x.to(BF16), *ops.quant_mxfp4(w), N)
@@ -255,7 +259,7 @@ def test_zero_rows_give_the_bias(ops):
 
 
 def test_captured_replayed_and_on_another_stream(ops):
-    for M in (1, 20, 300):
+    for M in (1, 20, 300, 1500):
         x, w, b = matrices(M, 640, 512)
         wq, ws = ops.quant_mxfp4(w)
         dy = torch.randn(M, 640, device=DEV).to(BF16)
