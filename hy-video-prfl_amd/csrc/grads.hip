@@ -11,6 +11,9 @@
 // for that would cost a small list a third of its time): no atomics, the same bits every time.
 #include <math.h>
 
+#include <algorithm>
+#include <vector>
+
 #include "common.h"
 
 namespace {
@@ -230,6 +233,26 @@ extern "C" int64_t prfl_grads_parts(const int64_t* n, int64_t count) {
   // a launch ends after PER tensors or 2^30 chunks
   const int64_t most = ((live + PER - 1) / PER + chunks / (1 << 29)) * norm_grid(live);
   return chunks < most ? chunks : most;
+}
+
+extern "C" int prfl_grads_overlap(const void* const* grads, const int64_t* n, const int32_t* type, int64_t count) {
+  if (count <= 0 || !grads || !n || !type) return 0;
+  try {
+    std::vector<uintptr_t> start, end;
+    for (int64_t i = 0; i < count; ++i)
+      if (n[i] > 0) {
+        start.push_back((uintptr_t)grads[i]);
+        end.push_back(start.back() + (uintptr_t)n[i] * (type[i] ? 2 : 4));
+      }
+    std::sort(start.begin(), start.end());
+    std::sort(end.begin(), end.end());
+    // apart if and only if the i-th end is not past the start after the i-th
+    for (size_t i = 0; i + 1 < start.size(); ++i)
+      if (end[i] > start[i + 1]) return 1;
+  } catch (...) {
+    return 1;                       // no memory for the lists
+  }
+  return 0;
 }
 
 extern "C" int prfl_grads_sumsq(const void* const* grads, const int64_t* n, const int32_t* type,

@@ -295,6 +295,112 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void mx_rows_kernel(MxArgs a, cons
   }
 }
 
+// dx = dy W for few rows, or few columns of W: 32 MT rows (MT 1 or 2; blockIdx.y) x one block of 32 columns of dx
+// per workgroup, its 16 waves taking every 16th 64 rows n of W, joined through LDS in wave order.  A lane holds
+// a row's block of 32 codes; the sum runs over rows, so the wave turns its 64 x 32 through LDS as bf16 (exact) for
+// the bf16 MFMA.  dy is rounded to bf16 on its way.  One launch, W read once per row group in four bits, no W in
+// bf16 in memory.
+constexpr int DX_PITCH = 80;              // bytes of a row of 32 bf16 in LDS: 16-byte accesses of 16 rows meet no bank twice
+
+template <typename T, int MT>
+__global__ __launch_bounds__(64 * ROWS_WAVES) void mx_dx_rows_kernel(const T* __restrict__ dy, int64_t lddy,
+                                                                     const uint8_t* __restrict__ wq,
+                                                                     const uint8_t* __restrict__ ws,
+                                                                     bf16* __restrict__ dx, int64_t lddx,
+                                                                     int64_t rows, int N, int K, int steps) {
+  __shared__ __attribute__((aligned(16))) char smem[ROWS_WAVES * 64 * DX_PITCH];
+  const int lane = threadIdx.x & 63, blk = lane >> 5;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kb = blockIdx.x, pieces = (N + 63) / 64;
+  const int64_t g = blockIdx.y;
+  const int M = (int)min(rows - g * 64, (int64_t)64);
+  // lane l takes row l of the piece
+  const int kl = (kb & 1) * 32 + (lane & 31), kh = (kb >> 1) & 1;
+  const uint8_t* w = wq + (int64_t)(kb >> 2) * PIECE + blk * 2048 + kh * 1024 + kl * 16;
+  const uint8_t* sw = ws + (int64_t)(kb >> 2) * PIECE_S + kl * 4 + blk * 2 + kh;
+  char* tile = smem + wid * 64 * DX_PITCH;
+  const char* turned = tile + (8 * blk + ((lane >> 2) & 3)) * DX_PITCH + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
+  f32x16 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = (f32x16)(0.f);
+  constexpr int AHEAD = 4;
+  u32x4 wv[AHEAD];
+  uint32_t sv[AHEAD];
+  for (int p0 = wid; p0 < pieces; p0 += AHEAD * ROWS_WAVES) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int64_t p = p0 + u * ROWS_WAVES;
+      if (p >= pieces) continue;
+      wv[u] = *(const u32x4*)(w + p * steps * PIECE);
+      sv[u] = sw[p * steps * PIECE_S];
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int p = p0 + u * ROWS_WAVES;
+      if (p >= pieces) break;
+      bf16x8 d[MT][4];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int row = m * 32 + (lane & 31), n = p * 64 + e * 16 + blk * 8;
+          const T* s = dy + (g * 64 + row) * lddy + n;
+          const int have = row < M ? N - n : 0;
+          if (have >= 8) {
+            const typename Loaded<T, 8>::vec t = *(const typename Loaded<T, 8>::at*)s;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[m][e][i] = (bf16)(float)t[i];
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) d[m][e][i] = i < have ? (bf16)(float)s[i] : (bf16)0.f;
+          }
+        }
+      const float scale = scale_value(sv[u]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        bf16x8 t;
+        const uint32_t c = wv[u][i];
+        const auto a0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 0);
+        const auto a1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 1);
+        const auto a2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 2);
+        const auto a3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 3);
+        t[0] = (bf16)(a0[0] * scale), t[1] = (bf16)(a0[1] * scale), t[2] = (bf16)(a1[0] * scale);
+        t[3] = (bf16)(a1[1] * scale), t[4] = (bf16)(a2[0] * scale), t[5] = (bf16)(a2[1] * scale);
+        t[6] = (bf16)(a3[0] * scale), t[7] = (bf16)(a3[1] * scale);
+        *(bf16x8*)(tile + lane * DX_PITCH + i * 16) = t;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const bf16x8 t = cat8(lds_read_tr(turned + e * 16 * DX_PITCH), lds_read_tr(turned + (e * 16 + 4) * DX_PITCH));
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[m] = mfma32(t, d[m][e], acc[m]);
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+  }
+  // register 4 q + c of lane l is column 8 q + 4 (l / 32) + c of row l % 32
+  float* part = (float*)smem;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) {
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const f32x4 v = {acc[m][4 * q], acc[m][4 * q + 1], acc[m][4 * q + 2], acc[m][4 * q + 3]};
+      *(f32x4*)(part + wid * 1024 + q * 256 + lane * 4) = v;
+    }
+    __syncthreads();
+    const int t = threadIdx.x, l = (t >> 2) & 63, mm = m * 32 + (l & 31);
+    const int k = kb * 32 + 8 * (t >> 8) + 4 * (l >> 5) + (t & 3);
+    if (mm < M && k < K) {
+      float s = 0.f;
+#pragma unroll
+      for (int i = 0; i < ROWS_WAVES; ++i) s += part[i * 1024 + t];
+      dx[(g * 64 + mm) * lddx + k] = f2bf(s);
+    }
+  }
+}
+
 // The tiled product: 64 WT x 64 WT of y per workgroup, four waves of 32 WT x 32 WT each.  Every step of
 // 128 columns (PIECE bytes a row piece) lands in a four-slot LDS ring by LDS-DMA, three steps ahead;
 // operands are in MFMA order already, so a piece is copied as it lies and every fragment is one
@@ -527,6 +633,13 @@ void launch_product(const MxArgs& a, hipStream_t st) {
 // one row: 5.2 us against 4.3 + 4.3 in two launches).
 bool fused(int64_t M, int64_t K) { return M <= 32 && M * ((K + 31) / 32) <= ROWS_FUSED; }
 
+// dx in one launch while its workgroups are few: kernel times in us against W read back to bf16 and multiplied by the
+// tiled bf16 product (M x N x K): 1 x 5120 x 5120 10.8 / 84.8, 64 x 5120 x 5120 22 / 86, 128 (320 workgroups) 43 /
+// 87, 256 (640) 65 / 87; 2 x 13312 x 96 22 / 185; 512 x 1280 x 1280 (320) 15.6 / 26.3; 2048 x 640 x 640 (640) 16.1 /
+// 16.7; 512 x 640 x 5120 (1280) 25.9 / 19.3; 160 x 1280 x 13824 (1296) 37.5 / 35.2; 20560 x 32 x 1472 (14812) 195 / 30.
+// What bounds it is dy, which every workgroup reads whole.
+constexpr int DX_DIRECT = 640;
+
 bool too_large(int64_t rows, int64_t cols) {       // pieces are counted in 31 bits
   return rows < 0 || cols < 1 || cols > (1 << 24) ||
          ((rows + 63) / 64) * ((cols + 127) / 128) > 0x7fffffff;
@@ -630,6 +743,40 @@ extern "C" int prfl_linear_mxfp4(const void* x, int x_type, int64_t ldx, const v
   else
     hipLaunchKernelGGL((mx_rows_kernel<_Float16, 1, true>), cols, dim3(64 * ROWS_WAVES), 0, st, a, (const _Float16*)x,
                        ldx, (int)K);
+  prfl_prof::set_work(2.0 * M * N * K);
+  prfl_prof::end(KID_GEMM, st);
+  PRFL_LAUNCH_CHECK();
+  return 0;
+}
+
+extern "C" int prfl_linear_mxfp4_dx_direct(int64_t M, int64_t N, int64_t K) {
+  return M > 0 && N > 0 && K > 0 && ((M + 63) / 64) * ((K + 31) / 32) <= DX_DIRECT;
+}
+
+extern "C" int prfl_linear_mxfp4_dx(const void* dy, int y_type, int64_t lddy, const void* wq, const void* ws,
+                                    void* dx, int64_t lddx, int64_t M, int64_t N, int64_t K, void* stream) {
+  if (too_large(M, K) || too_large(N, K) || N < 1 || N > (1 << 24) || y_type < 0 || y_type > 2 ||
+      (M > 1 && (lddy < 0 || lddx < K)) || (M + 63) / 64 > 65535)
+    return (int)hipErrorInvalidValue;
+  if (M == 0) return 0;
+  if (!dy || !wq || !ws || !dx || ((uintptr_t)wq & 15)) return (int)hipErrorInvalidValue;
+  hipStream_t st = (hipStream_t)stream;
+  const dim3 grid((unsigned)((K + 31) / 32), (unsigned)((M + 63) / 64));
+  const int steps = (int)((K + 127) / 128);
+  auto run = [&](auto* p) {
+    if (M <= 32)
+      hipLaunchKernelGGL((mx_dx_rows_kernel<std::remove_const_t<std::remove_pointer_t<decltype(p)>>, 1>), grid,
+                         dim3(64 * ROWS_WAVES), 0, st, p, lddy, (const uint8_t*)wq, (const uint8_t*)ws, (bf16*)dx,
+                         lddx, M, (int)N, (int)K, steps);
+    else
+      hipLaunchKernelGGL((mx_dx_rows_kernel<std::remove_const_t<std::remove_pointer_t<decltype(p)>>, 2>), grid,
+                         dim3(64 * ROWS_WAVES), 0, st, p, lddy, (const uint8_t*)wq, (const uint8_t*)ws, (bf16*)dx,
+                         lddx, M, (int)N, (int)K, steps);
+  };
+  prfl_prof::begin(KID_GEMM, st);
+  if (y_type == 0) run((const float*)dy);
+  else if (y_type == 1) run((const bf16*)dy);
+  else run((const _Float16*)dy);
   prfl_prof::set_work(2.0 * M * N * K);
   prfl_prof::end(KID_GEMM, st);
   PRFL_LAUNCH_CHECK();

@@ -82,12 +82,15 @@ SIGNATURES = {
     "prfl_layer_norm_bwd": [P, I32, I64, P, I32, I64, P, P, I64, I64, P, I32, P, I64, P, P, P, P],
     "prfl_layer_norm_parts": [I64, I64, I32],
     "prfl_grads_parts": [P, I64],
+    "prfl_grads_overlap": [P, P, P, I64],
     "prfl_grads_sumsq": [P, P, P, I64, P, I64, P, P],
     "prfl_grads_clip": [P, P, P, P, I64, I32, P, P, I64, F32, F32, P, P],
     "prfl_quant_mxfp4": [P, I32, I64, I64, I64, P, P, P],
     "prfl_dequant_mxfp4": [P, P, I64, I64, P, I32, I64, P],
     "prfl_linear_mxfp4_ws_bytes": [I64, I64],
     "prfl_linear_mxfp4": [P, I32, I64, P, P, P, P, I64, I64, I64, I64, P, I64, P],
+    "prfl_linear_mxfp4_dx_direct": [I64, I64, I64],
+    "prfl_linear_mxfp4_dx": [P, I32, I64, P, P, P, I64, I64, I64, I64, P],
     "prfl_gemm_mxfp4": [P, P, P, P, P, P, I64, I64, I64, I64, P],
     "prfl_prof_enable": [I32],
     "prfl_prof_collect": [P, P, P, I32],

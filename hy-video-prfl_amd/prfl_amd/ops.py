@@ -3,7 +3,7 @@
 All tensors are 2-D row-major views ``[rows, cols]`` with unit column stride; row strides are
 passed through, so q/k/v slices of the fused QKV output need no copy.
 """
-import ctypes
+import array
 import math
 
 import torch
@@ -522,43 +522,49 @@ def _dense(t):
 
 
 def _grad_list(grads, what, disjoint):
-    """(addresses, sizes, type codes) of the tensors as host arrays"""
+    """(addresses, sizes, type codes) of the tensors as host arrays; whether all are contiguous.  (A call
+    over a few dozen small tensors is these lists' time: one pass of C calls per attribute.)"""
     if not grads:
         raise ValueError(f"{what}: no tensors")
-    _lib.require_gpu(grads[0])
     dev = grads[0].device
-    at, n, types = [], [], []
+    if dev.type != "cuda":
+        _lib.require_gpu(grads[0])
+    plain = False
+    try:
+        plain = all([t.is_contiguous() for t in grads])
+        at = array.array("Q", [t.data_ptr() for t in grads])
+        types = array.array("i", [TYPES[t.dtype] for t in grads])
+        ok = plain or all([_dense(t) for t in grads])
+    except (KeyError, RuntimeError):             # another type; sparse tensors have no address
+        ok = False
+    if not ok:
+        got = next((t for t in grads if t.dtype not in TYPES or t.layout is not torch.strided or not _dense(t)),
+                   grads[0])
+        raise ValueError(f"{what}: dense fp32, bf16 or fp16 tensors in memory, got {got.dtype} "
+                         f"{tuple(got.shape)}, {got.layout}")
     for t in grads:
-        code = TYPES.get(t.dtype)
-        if code is None or t.layout is not torch.strided or not (t.is_contiguous() or _dense(t)):
-            raise ValueError(f"{what}: dense fp32, bf16 or fp16 tensors, got {t.dtype} "
-                             f"{tuple(t.shape)}, {t.layout}")
         if t.device != dev:
             raise ValueError(f"{what}: tensors on {dev} and {t.device}")
-        at.append(t.data_ptr())
-        n.append(t.numel())
-        types.append(code)
-    if disjoint:
-        end = 0
-        for a, k, code in sorted(zip(at, n, types)):
-            if k:
-                if a < end:
-                    raise ValueError(f"{what}: two of the tensors share memory")
-                end = a + k * (2 if code else 4)
-    k = len(grads)
-    return (ctypes.c_void_p * k)(*at), (ctypes.c_int64 * k)(*n), (ctypes.c_int32 * k)(*types)
+    n = array.array("q", [t.numel() for t in grads])
+    if disjoint and _lib.load().prfl_grads_overlap(_host(at), _host(n), _host(types), len(grads)):
+        raise ValueError(f"{what}: two of the tensors share memory")
+    return at, n, types, plain
+
+
+def _host(a):
+    return a.buffer_info()[0]
 
 
 def grads_sumsq(grads):
     """Sum of the squares of all elements of a list of dense fp32 / bf16 / fp16 tensors: fp64 [1] on
     their device.  (Ranks that hold shards add theirs, then clip_grads(sumsq=...).)"""
     grads = list(grads)
-    at, n, types = _grad_list(grads, "grads_sumsq", False)
+    at, n, types, _ = _grad_list(grads, "grads_sumsq", False)
     dev, k = grads[0].device, len(grads)
-    parts = _lib.load().prfl_grads_parts(n, k)
+    parts = _lib.load().prfl_grads_parts(_host(n), k)
     part = torch.empty(parts, dtype=torch.float64, device=dev)
     out = torch.empty(1, dtype=torch.float64, device=dev)
-    _lib.call_on(dev, "prfl_grads_sumsq", at, n, types, k, part.data_ptr(), parts, out.data_ptr())
+    _lib.call_on(dev, "prfl_grads_sumsq", _host(at), _host(n), _host(types), k, part.data_ptr(), parts, out.data_ptr())
     return out
 
 
@@ -571,23 +577,25 @@ def clip_grads(grads, max_norm, eps=1e-6, out=None, sumsq=None):
     grads = list(grads)
     dst, otype, k = None, -1, len(grads)
     if out is None:
-        at, n, types = _grad_list(grads, "clip_grads", True)
+        at, n, types, _ = _grad_list(grads, "clip_grads", True)
     else:
         out = list(out)
-        if len(out) != k or any(o.shape != g.shape or o.stride() != g.stride()
-                                or o.dtype != out[0].dtype for o, g in zip(out, grads)):
+        if len(out) != k or [o.shape for o in out] != [g.shape for g in grads]:
             raise ValueError("clip_grads: out has the gradients' shapes and strides, and one type")
-        at, n, types = _grad_list(grads + out, "clip_grads", True)      # first k: the gradients
-        dst, otype = (ctypes.c_void_p * k)(*at[k:]), types[k]
+        at, n, types, plain = _grad_list(grads + out, "clip_grads", True)      # first k: the gradients
+        otype = types[k]
+        if types[k:].count(otype) != k or not (plain or all(o.stride() == g.stride() for o, g in zip(out, grads))):
+            raise ValueError("clip_grads: out has the gradients' shapes and strides, and one type")
+        dst = _host(at) + 8 * k
     dev = grads[0].device
     part, parts = None, 0
     if sumsq is None:
-        parts = _lib.load().prfl_grads_parts(n, k)
-        part = torch.empty(parts, dtype=torch.float64, device=dev)
+        parts = _lib.load().prfl_grads_parts(_host(n), k)
+        part = grads[0].new_empty(parts, dtype=torch.float64)
     elif sumsq.dtype != torch.float64 or sumsq.numel() != 1 or sumsq.device != dev:
         raise ValueError("clip_grads: sumsq is one fp64 value on the gradients' device")
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    _lib.call_on(dev, "prfl_grads_clip", at, dst, n, types, k, otype, _addr(sumsq), _addr(part), parts,
+    norm = grads[0].new_empty((), dtype=torch.float32)
+    _lib.call_on(dev, "prfl_grads_clip", _host(at), dst, _host(n), _host(types), k, otype, _addr(sumsq), _addr(part), parts,
                  max_norm, eps, norm.data_ptr())
     return norm
 
@@ -660,15 +668,20 @@ def linear_mxfp4(x, wq, ws, out_features, bias=None):
 
 def linear_mxfp4_dx(dy, wq, ws, in_features):
     """dx [..., K] bf16 = dy W of linear_mxfp4, x's quantisation taken as the identity: W is read
-    back to bf16 (exact) and multiplied on the bf16 MFMA.  dy [..., N] is taken in bf16."""
+    back to bf16 (exact) and multiplied on the bf16 MFMA, for small products in one launch.  dy [..., N] is
+    taken in bf16."""
     N, K = dy.shape[-1], in_features
     dev = _one_device("linear_mxfp4_dx", dy, wq, ws)
     _mx_check("linear_mxfp4_dx", wq, ws, N, K)
-    _type(dy.dtype, "linear_mxfp4_dx")
-    d = _rows(dy, N).to(BF16)
+    yt = _type(dy.dtype, "linear_mxfp4_dx")
+    d = _rows(dy, N)
     M, Np, Kp = d.shape[0], -(-N // 8) * 8, -(-K // 8) * 8
-    if M == 0:
-        return torch.empty(*dy.shape[:-1], K, dtype=BF16, device=dev)
+    if M == 0 or _lib.load().prfl_linear_mxfp4_dx_direct(M, N, K):
+        dx = dy.new_empty((*dy.shape[:-1], K), dtype=BF16)
+        _lib.call_on(dev, "prfl_linear_mxfp4_dx", d.data_ptr(), yt, d.stride(0), wq.data_ptr(),
+                     ws.data_ptr(), dx.data_ptr(), K, M, N, K)
+        return dx
+    d = d.to(BF16)
     # the bf16 product takes extents in eights: padding rows and columns of W read back as zeros
     w = dequant_mxfp4(wq, ws, Np, Kp)
     if Np != N:

@@ -300,6 +300,8 @@ int64_t prfl_layer_norm_parts(int64_t rows, int64_t C, int x_type);
  * part: workspace of prfl_grads_parts(n, count) doubles.  Ranks that hold shards of the gradients
  * add their sumsq before the clip. */
 int64_t prfl_grads_parts(const int64_t* n, int64_t count);
+/* 1 if two of the tensors share a byte (a clip in place, or into others, of such is not defined) */
+int prfl_grads_overlap(const void* const* grads, const int64_t* n, const int32_t* type, int64_t count);
 int prfl_grads_sumsq(const void* const* grads, const int64_t* n, const int32_t* type, int64_t count,
                      double* part, int64_t parts, double* sumsq, void* stream);
 /* g *= min(1, max_norm / (norm + eps)), norm = sqrt(sumsq[0]), or with sumsq == NULL the norm of
@@ -335,6 +337,12 @@ int64_t prfl_linear_mxfp4_ws_bytes(int64_t M, int64_t K);
 int prfl_linear_mxfp4(const void* x, int x_type, int64_t ldx, const void* wq, const void* ws,
                       const void* bias, void* y, int64_t ldy, int64_t M, int64_t N, int64_t K,
                       void* work, int64_t work_bytes, void* stream);
+/* dx [M][K] bf16 = dy W, dy [M][N] (y_type as x_type, rounded to bf16, row stride lddy), W [N][K] tiled: for
+ * products of few rows or columns, of which prfl_linear_mxfp4_dx_direct says 1 (any others are right, and
+ * slower than prfl_dequant_mxfp4 and prfl_gemm_bf16).  At most 65535 * 64 rows. */
+int prfl_linear_mxfp4_dx_direct(int64_t M, int64_t N, int64_t K);
+int prfl_linear_mxfp4_dx(const void* dy, int y_type, int64_t lddy, const void* wq, const void* ws, void* dx,
+                         int64_t lddx, int64_t M, int64_t N, int64_t K, void* stream);
 
 /* ---- FlowUniPC sampler update (bh2, order <= 2, x0-prediction) ----------------------------
  * Replaces the element-wise body of FlowUniPCMultistepScheduler.step

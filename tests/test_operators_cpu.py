@@ -132,10 +132,32 @@ def test_overlapping_gradients_are_refused(ops, monkeypatch):
     flat = torch.zeros(100)
     refuses(lambda: ops.clip_grads([flat, flat], 1.0))
     refuses(lambda: ops.clip_grads([flat[:50], flat[49:]], 1.0))
+    refuses(lambda: ops.clip_grads([flat[60:], flat[20:40], flat[:10], flat[39:50], flat[90:91]], 1.0))
     refuses(lambda: ops.clip_grads([flat[:50]], 1.0, out=[flat[20:70]]))
     refuses(lambda: ops.clip_grads([flat[:50]], 1.0, out=[flat[:50]]))
     refuses(lambda: ops.clip_grads([flat[:5]], 1.0, sumsq=torch.zeros(1)))
     refuses(lambda: ops.clip_grads([flat[:5]], 1.0, sumsq=torch.zeros(2, dtype=F64)))
+
+
+def test_gradients_apart_are_taken(ops, monkeypatch):
+    from prfl_amd import _lib
+    monkeypatch.setattr(_lib, "require_gpu", lambda *t: None)
+    calls = []
+    monkeypatch.setattr(_lib, "call_on", lambda *a: calls.append(a))
+    flat, half = torch.zeros(100), torch.zeros(64, dtype=BF16)
+    ops.clip_grads([flat[60:], flat[20:40].view(4, 5).t(), flat[:0], flat[:10], flat[40:60], half[1:33], half[33:]], 1.0)
+    ops.clip_grads([flat[:10], half[:8]], 1.0, out=[flat[10:20], flat[20:28]])
+    ops.clip_grads([flat[30:30], flat[:50]], 1.0, out=[flat[:0], flat[50:]])
+    assert len(calls) == 3
+
+
+def test_sparse_gradients_are_refused(ops, monkeypatch):
+    from prfl_amd import _lib
+    monkeypatch.setattr(_lib, "require_gpu", lambda *t: None)
+    monkeypatch.setattr(_lib, "call_on", lambda *a: pytest.fail("launched"))
+    refuses(lambda: ops.clip_grads([torch.zeros(3), torch.eye(3).to_sparse()], 1.0))
+    refuses(lambda: ops.grads_sumsq([torch.eye(3).to_sparse_csr()]))
+    refuses(lambda: ops.clip_grads([torch.zeros(3)], 1.0, out=[torch.zeros(3).to_sparse()]))
 
 
 def test_empty_list_of_gradients(ops):
@@ -188,6 +210,16 @@ def test_c_entries_refuse(ops):
                 dict(M=65, K=129, w=p, nb=2 * 2 * 4352 - 1), dict(M=65, K=129, w=p + 8, nb=2 * 2 * 4352)):
         assert lin(**bad) == 1, bad
     assert lin(M=0) == 0
+
+    ldx = lambda dy=p, t=0, ld=8, wq=p, ws=p, dx=p, lddx=32, M=2, N=8, K=32: lib.prfl_linear_mxfp4_dx(  # noqa: E731
+        dy, t, ld, wq, ws, dx, lddx, M, N, K, None)
+    for bad in (dict(dy=None), dict(t=3), dict(t=-1), dict(ld=-1), dict(wq=None), dict(wq=p + 8), dict(ws=None),
+                dict(dx=None), dict(lddx=31), dict(M=-1), dict(N=0), dict(K=0), dict(M=65536 * 64),
+                dict(N=(1 << 24) + 1), dict(K=(1 << 24) + 1)):
+        assert ldx(**bad) == 1, bad
+    assert ldx(M=0) == 0
+    direct = lib.prfl_linear_mxfp4_dx_direct
+    assert direct(1, 8, 32) == 1 and not (direct(0, 8, 32) or direct(1, 0, 32) or direct(32760, 5120, 5120))
 
     n, t = (ctypes.c_int64 * 2)(4, 5), (ctypes.c_int32 * 2)(0, 1)
     at, none = (ctypes.c_void_p * 2)(p, p), (ctypes.c_void_p * 2)(p, None)
