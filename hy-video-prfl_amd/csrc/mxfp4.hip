@@ -296,19 +296,28 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void mx_rows_kernel(MxArgs a, cons
 }
 
 // dx = dy W for few rows, or few columns of W: 32 MT rows (MT 1 or 2; blockIdx.y) x one block of 32 columns of dx
-// per workgroup, its 16 waves taking every 16th 64 rows n of W, joined through LDS in wave order.  A lane holds
-// a row's block of 32 codes; the sum runs over rows, so the wave turns its 64 x 32 through LDS as bf16 (exact) for
-// the bf16 MFMA.  dy is rounded to bf16 on its way.  One launch, W read once per row group in four bits, no W in
-// bf16 in memory.
+// per workgroup, its waves taking every 16th (MT 2: 8th) 64 rows n of W, joined through LDS in wave order.  A lane
+// holds a row's block of 32 codes; the sum runs over rows, so the wave turns its 64 x 32 through LDS as bf16
+// (exact) for the bf16 MFMA.  dy is rounded to bf16 on its way.  One launch, W read once per row group in four
+// bits, no W in bf16 in memory.
+// dy, which every workgroup reads whole, sets the time, so a wave loads whole rows of it, 128 B of eight rows an
+// instruction, and takes the operands from LDS: 64 x 5120 x 5120 16 us, 22 with the operands loaded as they are used (32
+// pieces of 32 B an instruction; 1599 x 7445 x 608, rows of odd length: 53 us against 149).  MT 2 with 16 waves,
+// whose registers then leave room for one workgroup a CU: 22 us; MT 1 with 8: 11.0 instead of 9.9 us (32 rows).  Loads
+// issued earlier, one or two pieces ahead of their use, are no faster.
 constexpr int DX_PITCH = 80;              // bytes of a row of 32 bf16 in LDS: 16-byte accesses of 16 rows meet no bank twice
+constexpr int DY_PITCH = 144;             // the same of a row of 64 bf16 of dy
+constexpr int dx_waves(int MT) { return MT == 1 ? 16 : 8; }
 
 template <typename T, int MT>
-__global__ __launch_bounds__(64 * ROWS_WAVES) void mx_dx_rows_kernel(const T* __restrict__ dy, int64_t lddy,
-                                                                     const uint8_t* __restrict__ wq,
-                                                                     const uint8_t* __restrict__ ws,
-                                                                     bf16* __restrict__ dx, int64_t lddx,
-                                                                     int64_t rows, int N, int K, int steps) {
-  __shared__ __attribute__((aligned(16))) char smem[ROWS_WAVES * 64 * DX_PITCH];
+__global__ __launch_bounds__(64 * dx_waves(MT)) void mx_dx_rows_kernel(const T* __restrict__ dy, int64_t lddy,
+                                                                   const uint8_t* __restrict__ wq,
+                                                                   const uint8_t* __restrict__ ws,
+                                                                   bf16* __restrict__ dx, int64_t lddx,
+                                                                   int64_t rows, int N, int K, int steps) {
+  constexpr int WAVES = dx_waves(MT);
+  constexpr int TILE = MT * 32 * DY_PITCH > 64 * DX_PITCH ? MT * 32 * DY_PITCH : 64 * DX_PITCH;
+  __shared__ __attribute__((aligned(16))) char smem[WAVES * TILE];
   const int lane = threadIdx.x & 63, blk = lane >> 5;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kb = blockIdx.x, pieces = (N + 63) / 64;
@@ -318,66 +327,76 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void mx_dx_rows_kernel(const T* __
   const int kl = (kb & 1) * 32 + (lane & 31), kh = (kb >> 1) & 1;
   const uint8_t* w = wq + (int64_t)(kb >> 2) * PIECE + blk * 2048 + kh * 1024 + kl * 16;
   const uint8_t* sw = ws + (int64_t)(kb >> 2) * PIECE_S + kl * 4 + blk * 2 + kh;
-  char* tile = smem + wid * 64 * DX_PITCH;
+  char* tile = smem + wid * TILE;
   const char* turned = tile + (8 * blk + ((lane >> 2) & 3)) * DX_PITCH + ((lane >> 4) & 1) * 32 + (lane & 3) * 8;
   f32x16 acc[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) acc[m] = (f32x16)(0.f);
-  constexpr int AHEAD = 4;
-  u32x4 wv[AHEAD];
-  uint32_t sv[AHEAD];
-  for (int p0 = wid; p0 < pieces; p0 += AHEAD * ROWS_WAVES) {
+  typedef typename Loaded<T, 8>::vec raw8;
+  u32x4 wv;
+  uint32_t sv;
+  raw8 d[MT * 4];
+  // dy in runs of whole rows: lane l loads columns 8 (l % 8) of row l / 8 of every eighth row
+  const T* s = dy + (g * 64 + (lane >> 3)) * lddy + (lane & 7) * 8;
+  auto load = [&](int p) {
+    if (p >= pieces) return;
+    wv = *(const u32x4*)(w + (int64_t)p * steps * PIECE);
+    sv = sw[(int64_t)p * steps * PIECE_S];
+    const int have = N - p * 64 - (lane & 7) * 8;
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const int64_t p = p0 + u * ROWS_WAVES;
-      if (p >= pieces) continue;
-      wv[u] = *(const u32x4*)(w + p * steps * PIECE);
-      sv[u] = sw[p * steps * PIECE_S];
-    }
+    for (int i = 0; i < MT * 4; ++i) {
+      if (i * 8 >= M) continue;
+      const T* q = s + i * 8 * lddy + p * 64;
+      if (i * 8 + (lane >> 3) >= M) {
+      } else if (have >= 8) {
+        d[i] = *(const typename Loaded<T, 8>::at*)q;
+      } else {
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      const int p = p0 + u * ROWS_WAVES;
-      if (p >= pieces) break;
-      bf16x8 d[MT][4];
-#pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int row = m * 32 + (lane & 31), n = p * 64 + e * 16 + blk * 8;
-          const T* s = dy + (g * 64 + row) * lddy + n;
-          const int have = row < M ? N - n : 0;
-          if (have >= 8) {
-            const typename Loaded<T, 8>::vec t = *(const typename Loaded<T, 8>::at*)s;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) d[m][e][i] = (bf16)(float)t[i];
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) d[m][e][i] = i < have ? (bf16)(float)s[i] : (bf16)0.f;
-          }
-        }
-      const float scale = scale_value(sv[u]);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        bf16x8 t;
-        const uint32_t c = wv[u][i];
-        const auto a0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 0);
-        const auto a1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 1);
-        const auto a2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 2);
-        const auto a3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 3);
-        t[0] = (bf16)(a0[0] * scale), t[1] = (bf16)(a0[1] * scale), t[2] = (bf16)(a1[0] * scale);
-        t[3] = (bf16)(a1[1] * scale), t[4] = (bf16)(a2[0] * scale), t[5] = (bf16)(a2[1] * scale);
-        t[6] = (bf16)(a3[0] * scale), t[7] = (bf16)(a3[1] * scale);
-        *(bf16x8*)(tile + lane * DX_PITCH + i * 16) = t;
+        for (int k = 0; k < 8; ++k) d[i][k] = k < have ? q[k] : (T)0.f;
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const bf16x8 t = cat8(lds_read_tr(turned + e * 16 * DX_PITCH), lds_read_tr(turned + (e * 16 + 4) * DX_PITCH));
-#pragma unroll
-        for (int m = 0; m < MT; ++m) acc[m] = mfma32(t, d[m][e], acc[m]);
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
+  };
+  load(wid);
+  for (int p = wid; p < pieces; p += WAVES) {
+#pragma unroll
+    for (int i = 0; i < MT * 4; ++i) {
+      if (i * 8 >= M) continue;
+      bf16x8 t;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) t[k] = (bf16)(float)d[i][k];
+      *(bf16x8*)(tile + (i * 8 + (lane >> 3)) * DY_PITCH + (lane & 7) * 16) = t;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    bf16x8 y[MT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        y[m][e] = *(const bf16x8*)(tile + (m * 32 + (lane & 31)) * DY_PITCH + e * 32 + blk * 16);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const float scale = scale_value(sv);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      bf16x8 t;
+      const uint32_t c = wv[i];
+      const auto a0 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 0);
+      const auto a1 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 1);
+      const auto a2 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 2);
+      const auto a3 = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 3);
+      t[0] = (bf16)(a0[0] * scale), t[1] = (bf16)(a0[1] * scale), t[2] = (bf16)(a1[0] * scale);
+      t[3] = (bf16)(a1[1] * scale), t[4] = (bf16)(a2[0] * scale), t[5] = (bf16)(a2[1] * scale);
+      t[6] = (bf16)(a3[0] * scale), t[7] = (bf16)(a3[1] * scale);
+      *(bf16x8*)(tile + lane * DX_PITCH + i * 16) = t;
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const bf16x8 t = cat8(lds_read_tr(turned + e * 16 * DX_PITCH), lds_read_tr(turned + (e * 16 + 4) * DX_PITCH));
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[m] = mfma32(t, y[m][e], acc[m]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    load(p + WAVES);
   }
   // register 4 q + c of lane l is column 8 q + 4 (l / 32) + c of row l % 32
   float* part = (float*)smem;
@@ -390,13 +409,15 @@ __global__ __launch_bounds__(64 * ROWS_WAVES) void mx_dx_rows_kernel(const T* __
       *(f32x4*)(part + wid * 1024 + q * 256 + lane * 4) = v;
     }
     __syncthreads();
-    const int t = threadIdx.x, l = (t >> 2) & 63, mm = m * 32 + (l & 31);
-    const int k = kb * 32 + 8 * (t >> 8) + 4 * (l >> 5) + (t & 3);
-    if (mm < M && k < K) {
-      float s = 0.f;
 #pragma unroll
-      for (int i = 0; i < ROWS_WAVES; ++i) s += part[i * 1024 + t];
-      dx[(g * 64 + mm) * lddx + k] = f2bf(s);
+    for (int t = threadIdx.x; t < 1024; t += 64 * WAVES) {
+      const int l = (t >> 2) & 63, mm = m * 32 + (l & 31), k = kb * 32 + 8 * (t >> 8) + 4 * (l >> 5) + (t & 3);
+      if (mm < M && k < K) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < WAVES; ++i) s += part[i * 1024 + t];
+        dx[(g * 64 + mm) * lddx + k] = f2bf(s);
+      }
     }
   }
 }
@@ -634,11 +655,10 @@ void launch_product(const MxArgs& a, hipStream_t st) {
 bool fused(int64_t M, int64_t K) { return M <= 32 && M * ((K + 31) / 32) <= ROWS_FUSED; }
 
 // dx in one launch while its workgroups are few: kernel times in us against W read back to bf16 and multiplied by the
-// tiled bf16 product (M x N x K): 1 x 5120 x 5120 10.8 / 84.8, 64 x 5120 x 5120 22 / 86, 128 (320 workgroups) 43 /
-// 87, 256 (640) 65 / 87; 2 x 13312 x 96 22 / 185; 512 x 1280 x 1280 (320) 15.6 / 26.3; 2048 x 640 x 640 (640) 16.1 /
-// 16.7; 512 x 640 x 5120 (1280) 25.9 / 19.3; 160 x 1280 x 13824 (1296) 37.5 / 35.2; 20560 x 32 x 1472 (14812) 195 / 30.
-// What bounds it is dy, which every workgroup reads whole.
-constexpr int DX_DIRECT = 640;
+// tiled bf16 product (M x N x K): 1 x 5120 x 5120 7.9 / 85, 64 x 5120 x 5120 16 / 86, 128 (320 workgroups) 31 / 87, 256
+// (640) 48 / 87; 2 x 13312 x 96 15 / 184; 512 x 1280 x 1280 (320) 12.2 / 26.3; 2048 x 640 x 640 (640) 13.5 / 16.8;
+// 512 x 640 x 5120 (1280) 21.8 / 19.1.
+constexpr int DX_DIRECT = 1024;
 
 bool too_large(int64_t rows, int64_t cols) {       // pieces are counted in 31 bits
   return rows < 0 || cols < 1 || cols > (1 << 24) ||
@@ -766,11 +786,11 @@ extern "C" int prfl_linear_mxfp4_dx(const void* dy, int y_type, int64_t lddy, co
   auto run = [&](auto* p) {
     if (M <= 32)
       hipLaunchKernelGGL((mx_dx_rows_kernel<std::remove_const_t<std::remove_pointer_t<decltype(p)>>, 1>), grid,
-                         dim3(64 * ROWS_WAVES), 0, st, p, lddy, (const uint8_t*)wq, (const uint8_t*)ws, (bf16*)dx,
+                         dim3(64 * dx_waves(1)), 0, st, p, lddy, (const uint8_t*)wq, (const uint8_t*)ws, (bf16*)dx,
                          lddx, M, (int)N, (int)K, steps);
     else
       hipLaunchKernelGGL((mx_dx_rows_kernel<std::remove_const_t<std::remove_pointer_t<decltype(p)>>, 2>), grid,
-                         dim3(64 * ROWS_WAVES), 0, st, p, lddy, (const uint8_t*)wq, (const uint8_t*)ws, (bf16*)dx,
+                         dim3(64 * dx_waves(2)), 0, st, p, lddy, (const uint8_t*)wq, (const uint8_t*)ws, (bf16*)dx,
                          lddx, M, (int)N, (int)K, steps);
   };
   prfl_prof::begin(KID_GEMM, st);

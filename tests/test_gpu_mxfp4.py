@@ -210,7 +210,8 @@ def test_linear_to_the_bit(ops, M, N, K):
 @pytest.mark.parametrize("M,N,K", [(1, 8, 32), (3, 100, 100), (33, 1280, 96), (300, 333, 260), (512, 640, 1000),
                                    (1, 1, 1), (2, 13312, 96), (1, 5120, 5120), (32, 65, 129), (33, 64, 33),
                                    (64, 1000, 640), (65, 4100, 31), (129, 257, 2049), (2000, 33, 200),
-                                   (2000, 200, 1100), (1030, 133, 1111), (8200, 64, 160), (40, 300, 16400)])
+                                   (2000, 200, 1100), (1030, 133, 1111), (8200, 64, 160), (40, 300, 16400),
+                                   (1500, 320, 1280), (4100, 97, 999)])
 def test_gradient_of_x(ops, M, N, K):
     """dx = dy W: K bf16 products a row, fp32 sums, one rounding"""
     _, w, _ = matrices(M, N, K)
@@ -224,6 +225,32 @@ def test_gradient_of_x(ops, M, N, K):
     wide = torch.zeros(M, N + 5, dtype=BF16, device=DEV)
     wide[:, 3:3 + N] = dy
     assert torch.equal(ops.linear_mxfp4_dx(wide[:, 3:3 + N], wq, ws, K), dx)
+    for t in (F32, F16):                       # taken in bf16
+        assert torch.equal(ops.linear_mxfp4_dx(dy.to(t), wq, ws, K), ops.linear_mxfp4_dx(dy.to(t).to(BF16), wq, ws, K))
+    same_row = dy[:1].expand(M, N)
+    assert torch.equal(ops.linear_mxfp4_dx(same_row, wq, ws, K), ops.linear_mxfp4_dx(same_row.contiguous(), wq, ws, K))
+
+
+def test_gradient_of_x_takes_what_a_row_holds(ops):
+    """one row's NaN or infinity reaches no other row; a NaN block of W reaches its columns of dx alone"""
+    _, w, _ = matrices(70, 300, 200)
+    wq, ws = ops.quant_mxfp4(w)
+    for M in (5, 40, 70, 4000):
+        dy = torch.randn(M, 300, generator=torch.Generator().manual_seed(M)).to(BF16).to(DEV)
+        want = ops.linear_mxfp4_dx(dy, wq, ws, 200)
+        bad = dy.clone()
+        bad[M // 2, 17] = math.nan
+        bad[M - 1, 299] = math.inf
+        got = ops.linear_mxfp4_dx(bad, wq, ws, 200)
+        keep = torch.ones(M, dtype=torch.bool, device=DEV)
+        keep[M // 2] = keep[M - 1] = False
+        assert torch.equal(got[keep], want[keep])
+        assert got[M // 2].isnan().all() and not got[M - 1].isfinite().any()
+    w[3, 40] = math.nan
+    wq, ws = ops.quant_mxfp4(w)
+    for M in (5, 70, 4000):
+        got = ops.linear_mxfp4_dx(torch.ones(M, 300, dtype=BF16, device=DEV), wq, ws, 200)
+        assert got[:, 32:64].isnan().all() and got[:, :32].isfinite().all() and got[:, 64:].isfinite().all()
 
 
 def test_leading_axes_and_strides(ops):
