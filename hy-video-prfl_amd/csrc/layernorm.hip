@@ -29,62 +29,104 @@ struct Raw {
 template <typename T>
 constexpr int CHUNK = 16 / sizeof(T);          // 16 bytes of x
 
-// N values from p, the first n of them real (the others 0)
-template <typename T, int N>
-__device__ __forceinline__ typename Raw<T, N>::vec load_raw(const T* p, int n) {
+// A lane's N columns start at `at`: its stripe's, or where the row ends inside or before that the row's last N
+// (negative in rows narrower than N).  Columns i < lo of them are another lane's (lo >= N: all of them); they
+// count as zeros and are not stored.  So every load is one whole vector inside the row: a lane that loaded its last
+// elements one by one into the same registers would first wait for the vectors that the other lanes
+// have under way, the next row's among them (backward of 20651 x 6080 bf16: 259 us so, 164 with whole vectors).
+struct Own {
+  int at, lo;
+};
+template <int N>
+__device__ __forceinline__ Own own_columns(int column, int C) {
+  const int at = min(column, C - N);
+  return {at, column - at};
+}
+template <typename T, int N, bool SHORT>
+__device__ __forceinline__ typename Raw<T, N>::vec load_raw(const T* row, const Own& o, int C) {
   typename Raw<T, N>::vec t;
-  if (n >= N) {
-    t = *(const typename Raw<T, N>::at*)p;
+  if (!SHORT || C >= N) {
+    t = *(const typename Raw<T, N>::at*)(row + o.at);
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) t[i] = i < n ? p[i] : (T)0.f;
+    for (int i = 0; i < N; ++i) t[i] = i >= o.lo ? row[o.at + i] : (T)0.f;
   }
   return t;
 }
-template <typename T, int N>
-__device__ __forceinline__ void store_n(T* p, int n, const float (&v)[N]) {
-  if (n >= N) {
+template <bool SHORT, typename T, int N>
+__device__ __forceinline__ void store_n(T* row, const Own& o, int C, const float (&v)[N]) {
+  if (!SHORT || C >= N) {
     typename Raw<T, N>::vec t;
 #pragma unroll
     for (int i = 0; i < N; ++i) t[i] = (T)v[i];
-    *(typename Raw<T, N>::at*)p = t;
+    if (o.lo < N) *(typename Raw<T, N>::at*)(row + o.at) = t;
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i)
-      if (i < n) p[i] = (T)v[i];
+      if (i >= o.lo) row[o.at + i] = (T)v[i];
   }
 }
-template <int N>
-__device__ __forceinline__ void load_any(const void* p, int type, int64_t at, int n, float (&v)[N]) {
+template <int NV, int N>
+__device__ __forceinline__ bool any_not_own(const Own (&own)[NV]) {
+  bool some = false;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) some |= own[j].lo > 0;
+  return __any(some);
+}
+template <int N, bool SHORT>
+__device__ __forceinline__ void load_any(const void* p, int type, const Own& o, int C, float (&v)[N]) {
   auto widen = [&](auto raw) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (float)raw[i];
   };
-  if (type == 0) widen(load_raw<float, N>((const float*)p + at, n));
-  else if (type == 1) widen(load_raw<bf16, N>((const bf16*)p + at, n));
-  else widen(load_raw<_Float16, N>((const _Float16*)p + at, n));
+  if (type == 0) widen(load_raw<float, N, SHORT>((const float*)p, o, C));
+  else if (type == 1) widen(load_raw<bf16, N, SHORT>((const bf16*)p, o, C));
+  else widen(load_raw<_Float16, N, SHORT>((const _Float16*)p, o, C));
 }
 
 // mean and rstd of a row held as v[NV][N] per thread.  Within a wave two passes over the
 // registers; across waves the partial sums of squares about the waves' own means are joined:
 //   M2 = sum_w M2_w + n_w (mu_w - mu)^2,
-// so a mean far from zero costs no digits.  red: the row's [waves][2] floats, double-buffered by
-// the caller so that one barrier a row is enough.
+// so a mean far from zero costs no digits.  red: the row's sums per wave, double-buffered by the caller so
+// that one barrier a row is enough; every 16 lanes join them for themselves.  Sums over lanes go by DPP and
+// lane swaps, not through LDS: a row's turn is a chain of them (32760 x 5120 bf16 forward: 130 us, 147 with
+// shuffles and a loop over the waves).
+template <int CTRL>
+__device__ __forceinline__ float add_dpp(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
 template <int LANES>
 __device__ __forceinline__ float row_sum(float v) {
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  v = add_dpp<0xb1>(v);            // quad_perm 1 0 3 2
+  v = add_dpp<0x4e>(v);            // quad_perm 2 3 0 1
+  v = add_dpp<0x141>(v);           // row_half_mirror
+  v = add_dpp<0x140>(v);           // row_mirror
+  if constexpr (LANES >= 32) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  if constexpr (LANES == 64) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
   return v;
 }
 template <int NV, int N, int LANES>
-__device__ __forceinline__ void row_stats(const float (&v)[NV][N], const int (&cnt)[NV], int C, int nw,
+__device__ __forceinline__ void row_stats(const float (&v)[NV][N], const Own (&own)[NV], bool ragged, int C, int nw,
                                           int wave_n, float eps, float* red, float& mean,
                                           float& rstd) {
   float s = 0.f;
+  if (ragged) {
 #pragma unroll
-  for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j)
 #pragma unroll
-    for (int i = 0; i < N; ++i) s += v[j][i];
+      for (int i = 0; i < N; ++i) s += i >= own[j].lo ? v[j][i] : 0.f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < N; ++i) s += v[j][i];
+  }
   s = row_sum<LANES>(s);
   const float mw = wave_n > 0 ? s / wave_n : 0.f;
   float q = 0.f;
@@ -92,39 +134,34 @@ __device__ __forceinline__ void row_stats(const float (&v)[NV][N], const int (&c
   for (int j = 0; j < NV; ++j)
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-      const float d = i < cnt[j] ? v[j][i] - mw : 0.f;
+      const float d = i >= own[j].lo ? v[j][i] - mw : 0.f;
       q += d * d;
     }
   q = row_sum<LANES>(q);
   if (nw == 1) {
     mean = mw;
   } else {
-    const int w = threadIdx.x >> 6;
+    const int w = threadIdx.x >> 6, l = threadIdx.x & 15;
     if ((threadIdx.x & 63) == 0) {
-      red[3 * w] = s;
-      red[3 * w + 1] = q;
-      red[3 * w + 2] = (float)wave_n;
+      red[w] = s;
+      red[MAXW + w] = q;
+      red[2 * MAXW + w] = (float)wave_n;
     }
     __syncthreads();
-    s = 0.f;
-    for (int i = 0; i < nw; ++i) s += red[3 * i];
-    mean = s / C;
-    q = 0.f;
-    for (int i = 0; i < nw; ++i) {
-      const float n = red[3 * i + 2];
-      const float d = n > 0.f ? red[3 * i] / n - mean : 0.f;
-      q += red[3 * i + 1] + n * d * d;
-    }
+    const bool some = l < nw;
+    const float si = some ? red[l] : 0.f, qi = some ? red[MAXW + l] : 0.f, n = some ? red[2 * MAXW + l] : 0.f;
+    mean = row_sum<16>(si) / C;
+    const float d = n > 0.f ? si / n - mean : 0.f;
+    q = row_sum<16>(qi + n * d * d);
   }
   rstd = 1.f / sqrtf(q / C + eps);
 }
 
 // One row per workgroup at a time (nw waves), or with nw == 1 per LANES lanes (64, or 32 / 16 for rows
 // of that many chunks: 4 to 16 rows per workgroup).  16 waves a CU hide each other's loads, reductions and
-// stores: 73920 x 5120 fp32 to bf16 takes 0.44 ms = 5.2 TB/s, with the next row's loads issued ahead
-// 0.54 ms, and with more workgroups 0.48 to 0.55 ms.  Only rows past 8192 elements (AHEAD), of which a CU holds one
-// at a time, load the next row ahead (8000 x 16384 fp32: 195 us, 215 without).
-template <typename TX, typename TY, int NV, int LANES, bool AHEAD>
+// stores: 73920 x 5120 fp32 to bf16 takes 0.43 ms = 5.2 TB/s; with 24 waves a CU 0.46 ms, with the next row's loads
+// issued ahead 0.47 ms (8000 x 16384 fp32: 184 us, 200 with them).
+template <typename TX, typename TY, int NV, int LANES>
 __global__ __launch_bounds__(MAXT) void layer_norm_fwd_kernel(
     const TX* __restrict__ x, int64_t ldx, int64_t rows, int C, const void* __restrict__ w,
     const void* __restrict__ b, int wtype, float eps, TY* __restrict__ y, int64_t ldy,
@@ -134,10 +171,11 @@ __global__ __launch_bounds__(MAXT) void layer_norm_fwd_kernel(
   const int T = nw * 64, per = nw == 1 ? NARROW / LANES : 1;
   const int t = nw == 1 ? threadIdx.x & (LANES - 1) : threadIdx.x;
   const int first = t & ~63;                       // the wave's first chunk in each stripe
-  int cnt[NV], wave_n = 0;
+  Own own[NV];
+  int wave_n = 0;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    cnt[j] = min(max(C - (t + j * T) * N, 0), N);
+    own[j] = own_columns<N>((t + j * T) * N, C);
     wave_n += min(max(C - (first + j * T) * N, 0), 64 * N);
   }
   float wv[NV][N], bv[NV][N];
@@ -145,34 +183,28 @@ __global__ __launch_bounds__(MAXT) void layer_norm_fwd_kernel(
   for (int j = 0; j < NV; ++j) {
 #pragma unroll
     for (int i = 0; i < N; ++i) wv[j][i] = 1.f, bv[j][i] = 0.f;
-    if (w) load_any<N>(w, wtype, (int64_t)(t + j * T) * N, cnt[j], wv[j]);
-    if (b) load_any<N>(b, wtype, (int64_t)(t + j * T) * N, cnt[j], bv[j]);
+    if (w) load_any<N, LANES == 16>(w, wtype, own[j], C, wv[j]);
+    if (b) load_any<N, LANES == 16>(b, wtype, own[j], C, bv[j]);
   }
   int64_t row = (int64_t)blockIdx.x * per + (nw == 1 ? threadIdx.x / LANES : 0);
   const int64_t stride = (int64_t)gridDim.x * per;
+  const bool ragged = any_not_own<NV, N>(own);
   typename Raw<TX, N>::vec xr[NV];
-  auto load = [&](int64_t r) {
-    if (r < rows) {
-#pragma unroll
-      for (int j = 0; j < NV; ++j) xr[j] = load_raw<TX, N>(x + r * ldx + (t + j * T) * N, cnt[j]);
-    }
-  };
-  if (AHEAD) load(row);
   for (int it = 0; row < rows; row += stride, ++it) {
-    if (!AHEAD) load(row);
     float v[NV][N], mean, rstd;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) xr[j] = load_raw<TX, N, LANES == 16>(x + row * ldx, own[j], C);
 #pragma unroll
     for (int j = 0; j < NV; ++j)
 #pragma unroll
       for (int i = 0; i < N; ++i) v[j][i] = (float)xr[j][i];
-    if (AHEAD) load(row + stride);
-    row_stats<NV, N, LANES>(v, cnt, C, nw, wave_n, eps, red[it & 1], mean, rstd);
+    row_stats<NV, N, LANES>(v, own, ragged, C, nw, wave_n, eps, red[it & 1], mean, rstd);
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
       float o[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) o[i] = fmaf((v[j][i] - mean) * rstd, wv[j][i], bv[j][i]);
-      store_n<TY, N>(y + row * ldy + (t + j * T) * N, cnt[j], o);
+      store_n<LANES == 16, TY, N>(y + row * ldy, own[j], C, o);
     }
     if (t == 0) {
       mean_out[row] = mean;
@@ -183,8 +215,8 @@ __global__ __launch_bounds__(MAXT) void layer_norm_fwd_kernel(
 
 // dx of each row and, where asked for, the workgroup's sums of dy xhat and dy over its rows
 // (part_w / part_b [gridDim.x][C]).  The sums take as many registers as a row, so 12 waves at most share a CU
-// and the next row's loads are issued ahead: 32760 x 5120 bf16 takes 0.20 ms = 4.9 TB/s (0.46 without)
-// (rows past 8192 elements, TMAX 1024: two registers sets of a row do not fit, each row is loaded when
+// and the next row's loads are issued ahead: 32760 x 5120 bf16 takes 0.18 ms = 5.6 TB/s (0.28 without)
+// (rows past 8192 elements, TMAX 1024: two register sets of a row do not fit, each row is loaded when
 // its turn comes).
 template <typename TX, typename TY, int NV, int LANES, int TMAX>
 __global__ __launch_bounds__(TMAX) void layer_norm_bwd_kernel(
@@ -200,17 +232,18 @@ __global__ __launch_bounds__(TMAX) void layer_norm_bwd_kernel(
   const int T = nw * 64, per = nw == 1 ? GROUPS : 1;
   const int t = nw == 1 ? threadIdx.x & (LANES - 1) : threadIdx.x, wv_id = threadIdx.x >> 6;
   const int group = threadIdx.x / LANES;
-  int cnt[NV];
+  Own own[NV];
   float wv[NV][N], sw[NV][N], sb[NV][N];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    cnt[j] = min(max(C - (t + j * T) * N, 0), N);
+    own[j] = own_columns<N>((t + j * T) * N, C);
 #pragma unroll
     for (int i = 0; i < N; ++i) wv[j][i] = 1.f, sw[j][i] = 0.f, sb[j][i] = 0.f;
-    if (w) load_any<N>(w, wtype, (int64_t)(t + j * T) * N, cnt[j], wv[j]);
+    if (w) load_any<N, LANES == 16>(w, wtype, own[j], C, wv[j]);
   }
   int64_t row = (int64_t)blockIdx.x * per + (nw == 1 ? group : 0);
   const int64_t stride = (int64_t)gridDim.x * per;
+  const bool ragged = any_not_own<NV, N>(own);
   typename Raw<TX, N>::vec xr[NV];
   typename Raw<TY, N>::vec gr[NV];
   float mean_next = 0.f, rstd_next = 0.f;
@@ -220,8 +253,8 @@ __global__ __launch_bounds__(TMAX) void layer_norm_bwd_kernel(
       rstd_next = rstd_in[r];
 #pragma unroll
       for (int j = 0; j < NV; ++j) {
-        xr[j] = load_raw<TX, N>(x + r * ldx + (t + j * T) * N, cnt[j]);
-        gr[j] = load_raw<TY, N>(dy + r * lddy + (t + j * T) * N, cnt[j]);
+        xr[j] = load_raw<TX, N, LANES == 16>(x + r * ldx, own[j], C);
+        gr[j] = load_raw<TY, N, LANES == 16>(dy + r * lddy, own[j], C);
       }
     }
   };
@@ -246,17 +279,33 @@ __global__ __launch_bounds__(TMAX) void layer_norm_bwd_kernel(
         sw[j][i] = fmaf(g[j][i], xh[j][i], sw[j][i]);
         sb[j][i] += g[j][i];
         g[j][i] *= wv[j][i];
-        s1 += g[j][i];
-        s2 = fmaf(g[j][i], xh[j][i], s2);
       }
+    if (ragged) {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          s1 += i >= own[j].lo ? g[j][i] : 0.f;
+          s2 += i >= own[j].lo ? g[j][i] * xh[j][i] : 0.f;
+        }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          s1 += g[j][i];
+          s2 = fmaf(g[j][i], xh[j][i], s2);
+        }
+    }
     s1 = row_sum<LANES>(s1);
     s2 = row_sum<LANES>(s2);
     if (nw > 1) {
       float* r = red[it & 1];
-      if ((threadIdx.x & 63) == 0) r[2 * wv_id] = s1, r[2 * wv_id + 1] = s2;
+      if ((threadIdx.x & 63) == 0) r[wv_id] = s1, r[MAXW + wv_id] = s2;
       __syncthreads();
-      s1 = s2 = 0.f;
-      for (int i = 0; i < nw; ++i) s1 += r[2 * i], s2 += r[2 * i + 1];
+      const int l = threadIdx.x & 15;
+      s1 = row_sum<16>(l < nw ? r[l] : 0.f);
+      s2 = row_sum<16>(l < nw ? r[MAXW + l] : 0.f);
     }
     const float m1 = s1 / C, m2 = s2 / C;
     if (dx) {
@@ -265,7 +314,7 @@ __global__ __launch_bounds__(TMAX) void layer_norm_bwd_kernel(
         float o[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) o[i] = rstd * (g[j][i] - m1 - xh[j][i] * m2);
-        store_n<TX, N>(dx + row * lddx + (t + j * T) * N, cnt[j], o);
+        store_n<LANES == 16, TX, N>(dx + row * lddx, own[j], C, o);
       }
     }
   }
@@ -285,7 +334,7 @@ __global__ __launch_bounds__(TMAX) void layer_norm_bwd_kernel(
         }
       }
       if (nw > 1 || group == 0)
-        store_n<float, N>(part + (int64_t)blockIdx.x * C + (t + j * T) * N, cnt[j], s[j]);
+        store_n<LANES == 16, float, N>(part + (int64_t)blockIdx.x * C, own[j], C, s[j]);
     }
   };
   if (part_w) put(part_w, sw);
@@ -330,12 +379,14 @@ struct Split {
   int64_t rows_at_once() const { return nw == 1 ? NARROW / lanes : 1; }
   int threads() const { return nw == 1 ? NARROW : nw * 64; }
 };
-// wide: threads a row may take before they take more than one chunk each.  The forward is fastest with few
-// waves a row (40000 x 2048 bf16: 62 us with 2 waves, 94 with 4), the backward with more, for its registers
-// (fp32 32760 x 1280: 92 us with 5 waves, 105 with 2).
-constexpr int FWD_WIDE = 128, BWD_WIDE = 512;
-Split split_for(int C, int x_type, int wide) {
+// wide: lanes a row may take before they take more than one chunk each.  The forward is fastest with one wave a
+// row where that holds it (60000 x 640 bf16: 27 us, 47 with two waves; 37117 x 592 fp32: 22 and 30).  So is the backward up
+// to three chunks a lane (60000 x 640 bf16: 44 us, 58 with two waves; 37117 x 592 fp32: 41 and 45); rows past that take
+// more waves, for its registers (32760 x 1280 fp32: 92 us with 5 waves, 98 with 2).
+constexpr int FWD_WIDE = 64, BWD_WIDE = 512;
+Split split_for(int C, int x_type, bool backward) {
   const int n = x_type ? 8 : 4, most = 16 / n, chunks = (C + n - 1) / n;
+  const int wide = !backward || chunks <= 64 * (most < 3 ? most : 3) ? FWD_WIDE : BWD_WIDE;
   int nv = 1;
   while (nv < most && chunks > wide * nv) ++nv;
   return {nv, chunks <= 16 ? 16 : chunks <= 32 ? 32 : 64, (chunks + 64 * nv - 1) / (64 * nv)};
@@ -346,12 +397,14 @@ int grid_for_rows(int64_t rows, const Split& s, int waves) {
   const int each = waves / (s.threads() / 64), most = 256 * (each < 1 ? 1 : each);
   return (int)(g < most ? g : most);
 }
-constexpr int FWD_WAVES = 16, FWD_NARROW_WAVES = 24, BWD_WAVES = 12;
-// The backward's workgroups each leave C partial sums: 256 of them (one a CU), and more where each still has
-// four turns (1003 x 1021 fp16: 13 us in 256 workgroups, 18 in 1003).
+constexpr int FWD_WAVES = 16, FWD_NARROW_WAVES = 24, BWD_WAVES = 12, BWD_WIDE_WAVES = 8;
+// The backward's rows of several waves and chunks are fastest with one workgroup a CU (20651 x 6080 bf16: 142 us, 155
+// with two), the others with 12 waves (37117 x 592 fp32: 45 us, 63 with 8).  Its workgroups each leave C partial
+// sums: 256 of them (one a CU), and more where each still has four turns (4000 x 256 bf16: 8.1 us in 256
+// workgroups, 9.4 in 500).
 int bwd_grid(int64_t rows, const Split& s) {
   if (!rows) return 0;
-  const int g = grid_for_rows(rows, s, BWD_WAVES);
+  const int g = grid_for_rows(rows, s, s.nv > 1 && s.nw > 1 ? BWD_WIDE_WAVES : BWD_WAVES);
   const int64_t turns = (rows + 4 * s.rows_at_once() - 1) / (4 * s.rows_at_once());
   return g <= 256 || turns >= g ? g : (int)(turns > 256 ? turns : 256);
 }
@@ -390,7 +443,7 @@ bool bad(int64_t rows, int64_t C, int xt, int yt, int wt) {
 
 extern "C" int64_t prfl_layer_norm_parts(int64_t rows, int64_t C, int x_type) {
   if (bad(rows, C, x_type, 0, 0)) return 0;
-  return bwd_grid(rows, split_for((int)C, x_type, BWD_WIDE));
+  return bwd_grid(rows, split_for((int)C, x_type, true));
 }
 
 extern "C" int prfl_layer_norm_fwd(const void* x, int x_type, int64_t ldx, int64_t rows, int64_t C,
@@ -401,18 +454,15 @@ extern "C" int prfl_layer_norm_fwd(const void* x, int x_type, int64_t ldx, int64
   if (rows == 0) return 0;
   if (!x || !y || !mean || !rstd) return (int)hipErrorInvalidValue;
   hipStream_t s = (hipStream_t)stream;
-  const Split sp = split_for((int)C, x_type, FWD_WIDE);
+  const Split sp = split_for((int)C, x_type, false);
   const int grid = grid_for_rows(rows, sp, sp.nw == 1 ? FWD_NARROW_WAVES : FWD_WAVES);
   prfl_prof::begin(KID_LN, s);
   by_types(x_type, y_type, [&](auto* tx, auto* ty) {
     using TX = std::remove_const_t<std::remove_pointer_t<decltype(tx)>>;
     using TY = std::remove_const_t<std::remove_pointer_t<decltype(ty)>>;
     by_split<16 / CHUNK<TX>>(sp, [&](auto nv, auto lanes) {
-      auto kernel = layer_norm_fwd_kernel<TX, TY, nv(), lanes(), false>;
-      if constexpr (nv() * CHUNK<TX> == 16)      // rows past 8192 elements: more than 8 waves
-        if (sp.nw > 8) kernel = layer_norm_fwd_kernel<TX, TY, nv(), lanes(), true>;
-      hipLaunchKernelGGL(kernel, dim3(grid), dim3(sp.threads()), 0, s, (const TX*)x, ldx, rows, (int)C, w, b,
-                         w_type, eps, (TY*)y, ldy, mean, rstd, sp.nw);
+      hipLaunchKernelGGL((layer_norm_fwd_kernel<TX, TY, nv(), lanes()>), dim3(grid), dim3(sp.threads()), 0, s,
+                         (const TX*)x, ldx, rows, (int)C, w, b, w_type, eps, (TY*)y, ldy, mean, rstd, sp.nw);
     });
   });
   prfl_prof::set_work((double)rows * C * ((x_type ? 2 : 4) + (y_type ? 2 : 4)));
@@ -429,7 +479,7 @@ extern "C" int prfl_layer_norm_bwd(const void* dy, int y_type, int64_t lddy, con
       ((dw || db) && !part) || (rows && (dx || dw || db) && (!dy || !x || !mean || !rstd)))
     return (int)hipErrorInvalidValue;
   hipStream_t s = (hipStream_t)stream;
-  const Split sp = split_for((int)C, x_type, BWD_WIDE);
+  const Split sp = split_for((int)C, x_type, true);
   const int grid = bwd_grid(rows, sp);
   float* pw = dw ? part : nullptr;
   float* pb = db ? part + (dw ? (int64_t)grid * C : 0) : nullptr;

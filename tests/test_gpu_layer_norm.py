@@ -10,6 +10,7 @@ more: A = 64 covers the chain.
   dw:  (rows + 64) u sum |dy xhat| + sum |dy| d;   db: (rows + 64) u sum |dy|
 """
 import itertools
+import math
 
 import pytest
 import torch
@@ -103,6 +104,40 @@ def test_types(ops, xt, yt):
 def test_widths(ops, C, xt):
     x, w, b, dy = inputs((5, C), xt, seed=C)
     check(ops, x, w, b, dy)
+
+
+# rows that end inside a lane's vector, at a wave's end, in its last chunk and one past it
+@pytest.mark.parametrize("xt,yt", ((F32, BF16), (BF16, BF16), (F16, F32)))
+@pytest.mark.parametrize("C", (4, 5, 6, 33, 127, 129, 250, 260, 500, 516, 519, 770, 776, 1031, 1288, 1540, 1654, 2056,
+                               4104, 5003, 6076, 8200, 12001))
+def test_rows_that_end_inside_a_vector(ops, C, xt, yt):
+    x, w, b, dy = inputs((21, C), xt, seed=C)
+    check(ops, x, w, b, dy, out_dtype=yt)
+    wide, _, _, dwide = inputs((13, C + 3), xt, seed=C + 1)
+    check(ops, wide[:, 2:C + 2], w, None, dwide[:, 1:C + 1])
+    y, m, r = ops.layer_norm_fwd(x, w, b, out_dtype=yt)
+    again = ops.layer_norm_fwd(x, w, b, out_dtype=yt)[0]
+    assert torch.equal(y, again)
+    for a, c in zip(ops.layer_norm_bwd(dy, x, m, r, w), ops.layer_norm_bwd(dy, x, m, r, w)):
+        assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("C", (5, 100, 517, 1654, 6076))
+def test_a_value_that_is_no_number_stays_in_its_row(ops, C):
+    x, w, b, dy = inputs((40, C), BF16, seed=C)
+    y0, m, r = ops.layer_norm_fwd(x, w, b)
+    dx0 = ops.layer_norm_bwd(dy, x, m, r, w)[0]
+    for col in (0, C // 2, C - 2, C - 1):
+        for v in (math.nan, math.inf, -math.inf):
+            bad, dbad = x.clone(), dy.clone()
+            bad[7, col], dbad[9, col] = v, v
+            y, m1, r1 = ops.layer_norm_fwd(bad, w, b)
+            assert y[7].isnan().all() and torch.equal(y[:7], y0[:7]) and torch.equal(y[8:], y0[8:])
+            dx, dw, db = ops.layer_norm_bwd(dbad, x, m, r, w)
+            assert not dx[9].isfinite().any()
+            assert torch.equal(dx[:9], dx0[:9]) and torch.equal(dx[10:], dx0[10:])
+            keep = torch.arange(C, device=DEV) != col
+            assert not db[col].isfinite() and dw[keep].isfinite().all() and db[keep].isfinite().all()
 
 
 @pytest.mark.parametrize("rows", (1, 2, 3, 4, 5, 511, 512, 513, 2047, 2049, 8200))
