@@ -433,10 +433,12 @@ __global__ __launch_bounds__(64 * dx_waves(MT)) void mx_dx_rows_kernel(const T* 
 // slot of step j-1 was read for MFMAs that precede this barrier in every wave.  Past the last
 // step the DMA fetches it again into a slot nobody reads, so the count is the same every step.
 //
-// WT 4: 32760 x 13824 x 5120 takes 1.16 ms = 4.0 PFLOP/s.  MFMAs alone on random operands run at 6.0 to 6.6 PFLOP/s (the
-// clock falls to 1.5 GHz); here they are busy 54 % of 1.74 GHz, beside 96 B a clock of LDS traffic of a
-// possible 128.  Measured and dropped: one workgroup per CU walking its tiles as one stream of steps, the
-// finished tile held in registers and stored during the next one's steps: 1.16 ms too.
+// WT 4: 32760 x 13824 x 5120 takes 1.10 ms = 4.2 PFLOP/s.  MFMAs alone on random operands run at 6.0 to 6.6 PFLOP/s (the
+// clock falls to 1.5 GHz); here they are busy 57 % of 1.78 GHz.  A tile takes 65 k cycles: first loads 2.9 k, 40 steps
+// of 1316 (1024 of MFMAs), image 3.7 k, stores 4.9 k, the next workgroup 1.3 k.  Power bounds it, not those cycles: measured
+// and dropped, 1.10 ms each, were one workgroup per CU walking its tiles as one stream of steps, the finished tile
+// stored during the next one's, and the 16 x 16 x 128 MFMAs (alone 13 % faster), at 1.90 GHz for more cycles.  With the
+// operands' DMA left out it takes 0.84 ms, with a few KiB of operands from L2 1.08.
 // WT 2: LDS sets the time, 48 KiB a step per CU against 256 cycles of MFMAs (512 x 5120 x 4096: 12 us, of which 5 us are
 // launch, first loads and stores).  Measured and dropped, no faster: an eight-slot ring, fragments read a whole
 // step ahead, and two groups of waves that share K.
