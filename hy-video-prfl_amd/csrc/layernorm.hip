@@ -401,9 +401,10 @@ constexpr int FWD_WAVES = 16, FWD_NARROW_WAVES = 24, BWD_WAVES = 12, BWD_WIDE_WA
 // The backward's rows of several waves and chunks are fastest with one workgroup a CU (20651 x 6080 bf16: 142 us, 155
 // with two), the others with 12 waves (37117 x 592 fp32: 45 us, 63 with 8).  Its workgroups each leave C partial
 // sums: 256 of them (one a CU), and more where each still has four turns (4000 x 256 bf16: 8.1 us in 256
-// workgroups, 9.4 in 500).
+// workgroups, 9.4 in 500).  Up to four turns go to a single workgroup, whose sums are dw and db: one launch less.
 int bwd_grid(int64_t rows, const Split& s) {
   if (!rows) return 0;
+  if (rows <= 4 * s.rows_at_once()) return 1;
   const int g = grid_for_rows(rows, s, s.nv > 1 && s.nw > 1 ? BWD_WIDE_WAVES : BWD_WAVES);
   const int64_t turns = (rows + 4 * s.rows_at_once() - 1) / (4 * s.rows_at_once());
   return g <= 256 || turns >= g ? g : (int)(turns > 256 ? turns : 256);
@@ -443,7 +444,8 @@ bool bad(int64_t rows, int64_t C, int xt, int yt, int wt) {
 
 extern "C" int64_t prfl_layer_norm_parts(int64_t rows, int64_t C, int x_type) {
   if (bad(rows, C, x_type, 0, 0)) return 0;
-  return bwd_grid(rows, split_for((int)C, x_type, true));
+  const int grid = bwd_grid(rows, split_for((int)C, x_type, true));
+  return grid > 1 ? grid : 0;
 }
 
 extern "C" int prfl_layer_norm_fwd(const void* x, int x_type, int64_t ldx, int64_t rows, int64_t C,
@@ -476,13 +478,14 @@ extern "C" int prfl_layer_norm_bwd(const void* dy, int y_type, int64_t lddy, con
                                    int64_t C, const void* w, int w_type, void* dx, int64_t lddx,
                                    float* dw, float* db, float* part, void* stream) {
   if (bad(rows, C, x_type, y_type, w_type) || (rows > 1 && (ldx < 0 || lddy < 0 || (dx && lddx < C))) ||
-      ((dw || db) && !part) || (rows && (dx || dw || db) && (!dy || !x || !mean || !rstd)))
+      (rows && (dx || dw || db) && (!dy || !x || !mean || !rstd)))
     return (int)hipErrorInvalidValue;
   hipStream_t s = (hipStream_t)stream;
   const Split sp = split_for((int)C, x_type, true);
   const int grid = bwd_grid(rows, sp);
-  float* pw = dw ? part : nullptr;
-  float* pb = db ? part + (dw ? (int64_t)grid * C : 0) : nullptr;
+  if (grid > 1 && (dw || db) && !part) return (int)hipErrorInvalidValue;
+  float* pw = grid <= 1 || !dw ? dw : part;
+  float* pb = grid <= 1 || !db ? db : part + (dw ? (int64_t)grid * C : 0);
   prfl_prof::begin(KID_LN, s);
   if (rows && (dx || dw || db)) {
     by_types(x_type, y_type, [&](auto* tx, auto* ty) {
@@ -498,7 +501,7 @@ extern "C" int prfl_layer_norm_bwd(const void* dy, int y_type, int64_t lddy, con
       });
     });
   }
-  if (dw || db)
+  if (grid != 1 && (dw || db))
     hipLaunchKernelGGL(layer_norm_dw_kernel, dim3((C + 15) / 16, 2), dim3(1024), 0, s, pw, pb, grid,
                        (int)C, dw, db);
   prfl_prof::set_work((double)rows * C * (2 * (x_type ? 2 : 4) + (y_type ? 2 : 4)));

@@ -111,6 +111,7 @@ _lib = None
 # the current stream's handle without building a torch.cuda.Stream (1.9 us of a 4 us launch)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
                       lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def load():
@@ -138,8 +139,11 @@ def call(name, *args):
 def call_on(device, name, *args):
     """call(name, *args, stream) on `device`'s current stream, whichever device is current."""
     index = device.index
-    if torch.cuda.current_device() == index:
-        return call(name, *args, _raw_stream(index))
+    if _current_device() == index:
+        rc = getattr(_lib or load(), name)(*args, _raw_stream(index))
+        if rc != 0:
+            raise RuntimeError(f"{name} failed with hipError {rc}")
+        return rc
     with torch.cuda.device(device):
         return call(name, *args, _raw_stream(index))
 

@@ -445,28 +445,34 @@ def _rows(t, C):
 def layer_norm_fwd(x, w=None, b=None, eps=1e-5, out_dtype=None):
     """LN over the last axis of x [..., C] (C <= 16384), times w plus b ([C] each, or None):
     returns (y in out_dtype or x's, mean, rstd fp32 of x's leading shape)."""
-    C = x.shape[-1] if x.dim() else 0
+    shape = x.shape
+    C = shape[-1] if shape else 0
     if not 1 <= C <= 16384:
-        raise ValueError(f"layer_norm: a last axis of 1 to 16384, got {tuple(x.shape)}")
+        raise ValueError(f"layer_norm: a last axis of 1 to 16384, got {tuple(shape)}")
     dev = _one_device("layer_norm", x, w, b)
     ydt = x.dtype if out_dtype is None else out_dtype
-    xt, yt, wt = _type(x.dtype, "layer_norm x"), _type(ydt, "layer_norm out_dtype"), 0
-    for v in (w, b):
-        if v is not None:
-            wt = _type(v.dtype, "layer_norm w")
-            if v.shape != (C,) or (w is not None and v.dtype != w.dtype):
-                raise ValueError(f"layer_norm: w and b are [{C}] of one type")
+    xt, yt, wt, pw, pb = _type(x.dtype, "layer_norm x"), _type(ydt, "layer_norm out_dtype"), 0, None, None
+    if w is not None:
+        wt = _type(w.dtype, "layer_norm w")
+        w = w.contiguous()
+        pw = w.data_ptr()
+    if b is not None:
+        wt = _type(b.dtype, "layer_norm w")
+        b = b.contiguous()
+        pb = b.data_ptr()
+    if ((w is not None and w.shape != (C,)) or (b is not None and b.shape != (C,))
+            or (pw is not None and pb is not None and w.dtype != b.dtype)):
+        raise ValueError(f"layer_norm: w and b are [{C}] of one type")
     if not eps >= 0:
         raise ValueError(f"layer_norm: eps is not negative, got {eps}")
-    w, b = (v if v is None else v.contiguous() for v in (w, b))
     x2 = _rows(x, C)
     L = x2.shape[0]
     # (new_empty and empty_like cost half of torch.empty(device=) on the host, a third of a short call)
-    y = torch.empty_like(x, dtype=ydt) if x.is_contiguous() else x.new_empty(x.shape, dtype=ydt)
-    mean = x.new_empty(L if x.dim() == 2 else x.shape[:-1], dtype=torch.float32)
+    y = torch.empty_like(x, dtype=ydt) if x.is_contiguous() else x.new_empty(shape, dtype=ydt)
+    mean = x.new_empty(L if len(shape) == 2 else shape[:-1], dtype=torch.float32)
     rstd = torch.empty_like(mean)
-    _lib.call_on(dev, "prfl_layer_norm_fwd", x2.data_ptr(), xt, x2.stride(0), L, C, _addr(w),
-                 _addr(b), wt, eps, y.data_ptr(), yt, C, mean.data_ptr(), rstd.data_ptr())
+    _lib.call_on(dev, "prfl_layer_norm_fwd", x2.data_ptr(), xt, x2.stride(0), L, C, pw, pb, wt, eps,
+                 y.data_ptr(), yt, C, mean.data_ptr(), rstd.data_ptr())
     return y, mean, rstd
 
 
@@ -500,7 +506,7 @@ def layer_norm_bwd(dy, x, mean, rstd, w=None, want_dx=True, want_dw=None, want_d
     part = None
     if want_dw or want_db:
         n = _lib.load().prfl_layer_norm_parts(L, C, xt)
-        part = mean.new_empty(max(1, n * C * (int(want_dw) + int(want_db))))
+        part = mean.new_empty(n * C * (int(want_dw) + int(want_db))) if n else None
     _lib.call_on(dev, "prfl_layer_norm_bwd", dy2.data_ptr(), yt, dy2.stride(0), x2.data_ptr(), xt,
                  x2.stride(0), mean.data_ptr(), rstd.data_ptr(), L, C, _addr(w), wt, _addr(dx), C,
                  _addr(dw), _addr(db), _addr(part))

@@ -283,7 +283,7 @@ int prfl_layer_norm_fwd(const void* x, int x_type, int64_t ldx, int64_t rows, in
                         int64_t ldy, float* mean, float* rstd, void* stream);
 /* dx (x_type) and, where the pointer is not NULL, dw = sum dy * xhat and db = sum dy (fp32 [C]).
  * part: caller-owned fp32 workspace of prfl_layer_norm_parts(rows, C, x_type) * C elements for
- * each of dw and db that is asked for (may be NULL if neither is).  dx may be NULL.  The sums run
+ * each of dw and db that is asked for (may be NULL if that is 0).  dx may be NULL.  The sums run
  * in a fixed order (no atomics).  rows == 0 writes dw and db as zeros. */
 int prfl_layer_norm_bwd(const void* dy, int y_type, int64_t lddy, const void* x, int x_type,
                         int64_t ldx, const float* mean, const float* rstd, int64_t rows, int64_t C,

@@ -140,9 +140,9 @@ def test_a_value_that_is_no_number_stays_in_its_row(ops, C):
             assert not db[col].isfinite() and dw[keep].isfinite().all() and db[keep].isfinite().all()
 
 
-@pytest.mark.parametrize("rows", (1, 2, 3, 4, 5, 511, 512, 513, 2047, 2049, 8200))
+@pytest.mark.parametrize("rows", (1, 2, 3, 4, 5, 15, 16, 17, 32, 33, 63, 64, 65, 511, 512, 513, 2047, 2049, 8200))
 def test_rows(ops, rows):
-    for C, t in ((64, F16), (1280, BF16)):
+    for C, t in ((64, F16), (200, BF16), (700, BF16), (1280, BF16), (5, F32)):
         x, w, b, dy = inputs((rows, C), t, seed=rows)
         check(ops, x, w, b, dy)
 

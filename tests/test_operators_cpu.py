@@ -183,7 +183,7 @@ def test_c_entries_refuse(ops):
     bwd = lambda **k: lib.prfl_layer_norm_bwd(  # noqa: E731
         *{**dict(dy=p, yt=0, lddy=32, x=p, xt=0, ldx=32, mean=p, rstd=p, rows=4, C=32, w=p, wt=0, dx=p,
                  lddx=32, dw=p, db=p, part=p, st=None), **k}.values())
-    for bad in (dict(part=None), dict(C=16385), dict(xt=3), dict(lddx=31), dict(dy=None), dict(rows=-1)):
+    for bad in (dict(part=None, rows=100), dict(C=16385), dict(xt=3), dict(lddx=31), dict(dy=None), dict(rows=-1)):
         assert bwd(**bad) == 1, bad
     assert lib.prfl_layer_norm_parts(-1, 32, 0) == 0 and lib.prfl_layer_norm_parts(4, 0, 0) == 0
 
