@@ -629,9 +629,12 @@ __global__ __launch_bounds__(NT, WT == 4 ? 1 : 2) void mx_gemm_tile_kernel(MxArg
 //     13.9 / 13.5    192 x 4096 10.5 / 12.0 (K 1280: 7.1 / 6.1)    256 x 1280 6.1 / 11.1    512 x 1280 10.3 / 11.7
 //     128 x 8192 (K 4096) 15.0 / 10.2    300 x 100 (K 14000) 9.4 / 25.8    768 x 1024 (K 13824) 21.0 / 27.5
 //     16 x 65536 (K 4096) 36 / 24
-//   the 256 tile from 432 of them on, nearly two rounds (256 / 128 tile): 4096 x 5120 (320 tiles) 76 / 64,
-//     5000 x 5120 (400) 79 / 81, 2048 x 13824 (432) 81 / 83, 6000 x 5120 (480) 84.5 / 93, 8190 x 5120 (640) 120 / 122,
-//     16000 x 5120 (1260) 213 / 234
+//   else the tile whose rounds of the chip take less: 256 tiles of 256 at a time take 8.5 + 0.82 us a step of K, 512 of
+//   128, two a CU, whose loads and stores overlap, 2.5 + 0.51 (256 / 128 tile; tiles of 256):
+//     4096 x 4096 (256) 43 / 47 (K 1280: 18.3 / 17.4)    4352 x 5120 (340) 74 / 68    2048 x 13824 (432) 81 / 83    6000 x 5120
+//     (480) 84.5 / 93    7258 x 4808 (551) 132 / 125 (K 1280: 58 / 48)    8190 x 5120 (640) 120 / 122    6400 x 8192 (800)
+//     166 / 169 (K 640: 47 / 35)    8960 x 7680 (1050) 210 / 221    16000 x 5120 (1260) 213 / 234
+//     12359 x 2272, K 1760 (441) 47 / 39    17996 x 9984, K 1792 (2769) 240 / 248
 bool by_rows(int64_t M, int64_t N, int steps) {
   const int64_t n = ((M + 63) / 64) * ((N + 31) / 32);
   return n <= 256 || (n <= 384 && steps >= 20) || (M <= 32 && n <= 512);
@@ -639,13 +642,14 @@ bool by_rows(int64_t M, int64_t N, int steps) {
 
 void launch_product(const MxArgs& a, hipStream_t st) {
   const int64_t t256 = ((a.M + 255) / 256) * ((a.N + 255) / 256), t128 = ((a.M + 127) / 128) * ((a.N + 127) / 128);
+  const int64_t us256 = ((t256 + 255) / 256) * (850 + 82 * a.steps), us128 = ((t128 + 511) / 512) * (250 + 51 * a.steps);
   const dim3 cols((unsigned)((a.N + 31) / 32), (unsigned)((a.M + 63) / 64));
   if (by_rows(a.M, a.N, a.steps)) {
     if (a.M <= 32)
       hipLaunchKernelGGL((mx_rows_kernel<bf16, 1, false>), cols, dim3(64 * ROWS_WAVES), 0, st, a, nullptr, 0, 0);
     else
       hipLaunchKernelGGL((mx_rows_kernel<bf16, 2, false>), cols, dim3(64 * ROWS_WAVES), 0, st, a, nullptr, 0, 0);
-  } else if (t256 >= 432) {
+  } else if (us256 < us128) {
     hipLaunchKernelGGL(mx_gemm_tile_kernel<4>, dim3((unsigned)t256), dim3(NT), 0, st, a);
   } else {
     hipLaunchKernelGGL(mx_gemm_tile_kernel<2>, dim3((unsigned)t128), dim3(NT), 0, st, a);

@@ -200,7 +200,8 @@ def exact_matrices(M, N, K, seed=0):
 @pytest.mark.parametrize("M,N,K", [(1, 160, 5120), (3, 512, 1024), (17, 96, 640), (40, 130, 2048),
                                    (130, 258, 4096), (300, 200, 5120), (512, 512, 128), (770, 1030, 1152),
                                    (6, 320, 5120), (64, 320, 2200), (5500, 5632, 640), (5500, 5600, 384),
-                                   (512, 1280, 2688), (384, 2048, 640), (1023, 129, 4100), (12, 16500, 300)])
+                                   (512, 1280, 2688), (384, 2048, 640), (1023, 129, 4100), (12, 16500, 300),
+                                   (4096, 4096, 5120), (3900, 4000, 5000), (4091, 3975, 5003), (4095, 4097, 8192)])
 def test_linear_to_the_bit(ops, M, N, K):
     x, w = exact_matrices(M, N, K)
     y = ops.linear_mxfp4(x.to(BF16), *ops.quant_mxfp4(w), N)

@@ -61,13 +61,15 @@ def test_quantise_and_read_back(ops, big):
 
 
 def test_linear(ops, big):
-    """y of 2.15e9 elements: the tiles of the last 8192 rows are those of a call on them"""
-    x = big.view(-1)[:ROWS * 96].view(ROWS, 96)
-    wq, ws = ops.quant_mxfp4(torch.randn(COLS, 96, device=DEV))
+    """x and y of 2.15e9 elements, with a short and a long K: the last 8192 rows are those of a call on them
+    (every tile adds K in the same order)"""
     b = torch.randn(COLS, device=DEV).to(BF16)
-    y = ops.linear_mxfp4(x, wq, ws, COLS, b)
-    assert torch.equal(y[-8192:], ops.linear_mxfp4(x[-8192:], wq, ws, COLS, b))
-    assert torch.equal(y[:8192], ops.linear_mxfp4(x[:8192], wq, ws, COLS, b))
+    for k in (96, COLS):
+        x = big.view(-1)[:ROWS * k].view(ROWS, k)
+        wq, ws = ops.quant_mxfp4(torch.randn(COLS, k, device=DEV))
+        y = ops.linear_mxfp4(x, wq, ws, COLS, b)
+        assert torch.equal(y[-8192:], ops.linear_mxfp4(x[-8192:], wq, ws, COLS, b))
+        assert torch.equal(y[:8192], ops.linear_mxfp4(x[:8192], wq, ws, COLS, b))
 
 
 def test_linear_of_far_rows(ops, big):
