@@ -663,7 +663,8 @@ bool fused(int64_t M, int64_t K) { return M <= 32 && M * ((K + 31) / 32) <= ROWS
 // dx in one launch while its workgroups are few: kernel times in us against W read back to bf16 and multiplied by the
 // tiled bf16 product (M x N x K): 1 x 5120 x 5120 7.9 / 85, 64 x 5120 x 5120 16 / 86, 128 (320 workgroups) 31 / 87, 256
 // (640) 48 / 87; 2 x 13312 x 96 15 / 184; 512 x 1280 x 1280 (320) 12.2 / 26.3; 2048 x 640 x 640 (640) 13.5 / 16.8;
-// 512 x 640 x 5120 (1280) 21.8 / 19.1.
+// 512 x 13824 x 4000 (1000) 163 / 215; 512 x 640 x 5120 (1280) 21.8 / 19.1.  A single group of 64 rows reads W once either
+// way, here in four bits, and stays here whatever its width: 64 x 14000 x 13824 83 / 335, 32 x 8192 x 30000 54 / 304.
 constexpr int DX_DIRECT = 1024;
 
 bool too_large(int64_t rows, int64_t cols) {       // pieces are counted in 31 bits
@@ -776,7 +777,7 @@ extern "C" int prfl_linear_mxfp4(const void* x, int x_type, int64_t ldx, const v
 }
 
 extern "C" int prfl_linear_mxfp4_dx_direct(int64_t M, int64_t N, int64_t K) {
-  return M > 0 && N > 0 && K > 0 && ((M + 63) / 64) * ((K + 31) / 32) <= DX_DIRECT;
+  return M > 0 && N > 0 && K > 0 && (M <= 64 || ((M + 63) / 64) * ((K + 31) / 32) <= DX_DIRECT);
 }
 
 extern "C" int prfl_linear_mxfp4_dx(const void* dy, int y_type, int64_t lddy, const void* wq, const void* ws,

@@ -212,7 +212,7 @@ def test_linear_to_the_bit(ops, M, N, K):
                                    (1, 1, 1), (2, 13312, 96), (1, 5120, 5120), (32, 65, 129), (33, 64, 33),
                                    (64, 1000, 640), (65, 4100, 31), (129, 257, 2049), (2000, 33, 200),
                                    (2000, 200, 1100), (1030, 133, 1111), (8200, 64, 160), (40, 300, 16400),
-                                   (1500, 320, 1280), (4100, 97, 999)])
+                                   (1500, 320, 1280), (4100, 97, 999), (3, 64, 40000), (64, 70, 33000)])
 def test_gradient_of_x(ops, M, N, K):
     """dx = dy W: K bf16 products a row, fp32 sums, one rounding"""
     _, w, _ = matrices(M, N, K)
