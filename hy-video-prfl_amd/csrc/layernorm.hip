@@ -400,14 +400,15 @@ int grid_for_rows(int64_t rows, const Split& s, int waves) {
 constexpr int FWD_WAVES = 16, FWD_NARROW_WAVES = 24, BWD_WAVES = 12, BWD_WIDE_WAVES = 8;
 // The backward's rows of several waves and chunks are fastest with one workgroup a CU (20651 x 6080 bf16: 142 us, 155
 // with two), the others with 12 waves (37117 x 592 fp32: 45 us, 63 with 8).  Its workgroups each leave C partial
-// sums: 256 of them (one a CU), and more where each still has four turns (4000 x 256 bf16: 8.1 us in 256
-// workgroups, 9.4 in 500).  Up to four turns go to a single workgroup, whose sums are dw and db: one launch less.
+// sums: 128 of them, and more where each still has four turns (300 x 16384 bf16: 22.5 us in 128 workgroups, 27.6 in
+// 256; 400 x 5120: 14.6 and 18.0; 4000 x 256: 8.4, 7.9 in 256, 9.4 in 500).  Up to four turns go to a single
+// workgroup, whose sums are dw and db: one launch less.
 int bwd_grid(int64_t rows, const Split& s) {
   if (!rows) return 0;
   if (rows <= 4 * s.rows_at_once()) return 1;
   const int g = grid_for_rows(rows, s, s.nv > 1 && s.nw > 1 ? BWD_WIDE_WAVES : BWD_WAVES);
   const int64_t turns = (rows + 4 * s.rows_at_once() - 1) / (4 * s.rows_at_once());
-  return g <= 256 || turns >= g ? g : (int)(turns > 256 ? turns : 256);
+  return g <= 128 || turns >= g ? g : (int)(turns > 128 ? turns : 128);
 }
 
 template <typename F>
