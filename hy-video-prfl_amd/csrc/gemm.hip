@@ -1362,12 +1362,14 @@ int launch(const GemmArgs& g, hipStream_t s, int tile) {
     hipLaunchKernelGGL((gemm256s_kernel<A_KC, B_KC, EPI>), dim3(nt256), dim3(NT2), 0, s, g);
   } else if (tile == 256 || (tile == 0 && fits256 && nt256 >= 96)) {
     // the four-wave kernel (each operand addressed through a 32-bit buffer offset) wherever
-    // the operands fit 4 GiB; the 8-wave kernel otherwise (and for the epilogues switched back
-    // by GEMM_GELU_4W / GEMM_RESID_4W = 0)
+    // the operands fit 4 GiB and their rows lie apart: its buffer covers rows * stride elements, so of rows
+    // that share memory (a broadcast gradient has stride 0) it would read zeros.  The 8-wave kernel, which
+    // addresses by pointer, otherwise (and for the epilogues switched back by GEMM_GELU_4W / GEMM_RESID_4W = 0)
     const int64_t bytes_a = (A_KC ? (int64_t)g.M : (int64_t)g.K) * g.lda * 2;
     const int64_t bytes_b = (B_KC ? (int64_t)g.N : (int64_t)g.K) * g.ldb * 2;
     const bool four = (GEMM_GELU_4W || EPI != EPI_GELU) && (GEMM_RESID_4W || EPI != EPI_RESID) &&
-                      bytes_a < (1ll << 32) && bytes_b < (1ll << 32);
+                      bytes_a < (1ll << 32) && bytes_b < (1ll << 32) &&
+                      g.lda >= (A_KC ? g.K : g.M) && g.ldb >= (B_KC ? g.K : g.N);
     if (four && (GEMM_MFMA32 || (EPI == EPI_F32 && !A_KC && !B_KC)))
       hipLaunchKernelGGL((gemm4x_kernel<A_KC, B_KC, EPI>), dim3(nt256), dim3(256), 0, s, g);
     else if (four)
