@@ -603,6 +603,10 @@ def clip_grads(grads, max_norm, eps=1e-6, out=None, sumsq=None):
     norm = grads[0].new_empty((), dtype=torch.float32)
     _lib.call_on(dev, "prfl_grads_clip", _host(at), dst, _host(n), _host(types), k, otype, _addr(sumsq), _addr(part), parts,
                  max_norm, eps, norm.data_ptr())
+    if out is not None:
+        # written: AdamW and autograd read it off the version counter.  (In place the counter stays, as it does
+        # for scale_: a gradient that AdamW zeroed and that received nothing since is still none after it.)
+        torch.autograd.graph.increment_version(out)
     return norm
 
 

@@ -151,6 +151,17 @@ def test_gradients_apart_are_taken(ops, monkeypatch):
     assert len(calls) == 3
 
 
+def test_tensors_clipped_into_count_as_written(ops, monkeypatch):
+    from prfl_amd import _lib
+    monkeypatch.setattr(_lib, "require_gpu", lambda *t: None)
+    monkeypatch.setattr(_lib, "call_on", lambda *a: 0)
+    grads, out = [torch.ones(5, dtype=BF16), torch.ones(3, dtype=BF16)], [torch.zeros(5), torch.zeros(3)]
+    ops.clip_grads(grads, 1.0, out=out)
+    assert [t._version for t in grads + out] == [0, 0, 1, 1]
+    ops.clip_grads(grads, 1.0)
+    assert [t._version for t in grads] == [0, 0]
+
+
 def test_sparse_gradients_are_refused(ops, monkeypatch):
     from prfl_amd import _lib
     monkeypatch.setattr(_lib, "require_gpu", lambda *t: None)
