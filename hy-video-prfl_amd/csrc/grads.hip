@@ -112,11 +112,26 @@ __global__ __launch_bounds__(NT) void grads_norm_join_kernel(const double* __res
   if (threadIdx.x == 0) sumsq[0] = s;
 }
 
+// The factor as f * post, post a power of two.  It is formed in fp32 where that holds it (post 1); a norm past
+// the largest fp32 (gradients of 1e38) or a factor below its smallest normal number goes through 64 bits and keeps its
+// digits in f, since what it scales need not be small: 1e38 clipped to a norm of 1 is an ordinary number.
+struct Factor {
+  float f, post;
+};
+__device__ __forceinline__ Factor factor(double total, float max_norm, float eps) {
+  const float c = max_norm / ((float)total + eps);
+  if (c >= 0x1p-126f || !(total < __builtin_huge_val())) return {c > 1.f ? 1.f : c, 1.f};   // a NaN norm stays NaN
+  const double d = max_norm / (total + eps);
+  if (!(d < 1.0)) return {1.f, 1.f};               // and 0 / 0, whose gradients are all zeros
+  if (d >= 0x1p-126) return {(float)d, 1.f};
+  return {(float)(d * 0x1p126), 0x1p-126f};
+}
+
 // Vectors of 16 bytes of the wider type, so that a store instruction writes whole lines (bf16 to fp32
 // over 0.8 G elements: 1.18 ms with the norm, against 1.24 with 16-byte loads and two stores each),
 // four loads in flight per thread (one: 1.30 ms, eight: 1.19).
 template <typename TS, typename TD>
-__device__ __forceinline__ void scaled(const TS* src, TD* dst, int len, float f) {
+__device__ __forceinline__ void scaled(const TS* src, TD* dst, int len, Factor by) {
   constexpr int N = 16 / (sizeof(TS) > sizeof(TD) ? sizeof(TS) : sizeof(TD)), AHEAD = 4, STEP = NT * N;
   typedef TS svec __attribute__((ext_vector_type(N)));
   typedef svec sat __attribute__((aligned(sizeof(TS))));
@@ -131,39 +146,34 @@ __device__ __forceinline__ void scaled(const TS* src, TD* dst, int len, float f)
     for (int u = 0; u < AHEAD; ++u) {
       dvec o;
 #pragma unroll
-      for (int k = 0; k < N; ++k) o[k] = (TD)((float)v[u][k] * f);
+      for (int k = 0; k < N; ++k) o[k] = (TD)((float)v[u][k] * by.f * by.post);
       *(dat*)(dst + i + u * STEP) = o;
     }
   }
   for (; i < len; i += STEP)
-    for (int k = i; k < len && k < i + N; ++k) dst[k] = (TD)((float)src[k] * f);
+    for (int k = i; k < len && k < i + N; ++k) dst[k] = (TD)((float)src[k] * by.f * by.post);
 }
 
-__device__ __forceinline__ float coefficient(float norm, float max_norm, float eps) {
-  const float c = max_norm / (norm + eps);
-  return c > 1.f ? 1.f : c;         // a NaN norm stays NaN
-}
-
-// dst = src * coefficient; norm_out gets the norm once.  In place with a coefficient of 1 nothing
+// dst = src * factor; norm_out gets the norm once (infinity past fp32).  In place with a factor of 1 nothing
 // changes, so nothing is read.
 __global__ __launch_bounds__(NT) void grads_clip_kernel(Tensors t, int dtype,
                                                         const double* __restrict__ part, int P,
                                                         float max_norm, float eps,
                                                         float* __restrict__ norm_out) {
   __shared__ double red[NT / 64];
-  const float norm = (float)sqrt(sum_parts(part, P, red));
-  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = norm;
-  const float f = coefficient(norm, max_norm, eps);
-  if (dtype < 0 && f == 1.f) return;
+  const double total = sqrt(sum_parts(part, P, red));
+  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) norm_out[0] = (float)total;
+  const Factor by = factor(total, max_norm, eps);
+  if (dtype < 0 && by.f == 1.f && by.post == 1.f) return;
   for (int c = blockIdx.x; c < t.first[t.count]; c += gridDim.x) {
     const int i = owner(t, c);
     const int64_t n = t.n[i] & ((1ll << 60) - 1), at = (int64_t)(c - t.first[i]) * CHUNK;
     const int len = (int)(n - at < CHUNK ? n - at : CHUNK), type = (int)(t.n[i] >> 60);
     const int to = dtype < 0 ? type : dtype;
     auto run = [&](auto* src) {
-      if (to == 0) scaled(src + at, (float*)t.dst[i] + at, len, f);
-      else if (to == 1) scaled(src + at, (bf16*)t.dst[i] + at, len, f);
-      else scaled(src + at, (_Float16*)t.dst[i] + at, len, f);
+      if (to == 0) scaled(src + at, (float*)t.dst[i] + at, len, by);
+      else if (to == 1) scaled(src + at, (bf16*)t.dst[i] + at, len, by);
+      else scaled(src + at, (_Float16*)t.dst[i] + at, len, by);
     };
     if (type == 0) run((const float*)t.src[i]);
     else if (type == 1) run((const bf16*)t.src[i]);

@@ -577,7 +577,8 @@ def grads_sumsq(grads):
 def clip_grads(grads, max_norm, eps=1e-6, out=None, sumsq=None):
     """Scale the tensors by min(1, max_norm / (norm + eps)), norm their global L2 norm (or
     sqrt(sumsq) where that is given); in place, or into `out`, a list of tensors of the same shapes
-    and one type.  Returns the norm before clipping, fp32 0-dim on the device (nothing waits)."""
+    and one type.  Returns the norm before clipping, fp32 0-dim on the device (nothing waits; infinity
+    where it is past fp32, which the clipped values do not suffer from)."""
     if not max_norm >= 0 or not eps >= 0:
         raise ValueError(f"clip_grads: max_norm and eps are not negative, got {max_norm}, {eps}")
     grads = list(grads)

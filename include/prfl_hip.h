@@ -305,7 +305,8 @@ int prfl_grads_overlap(const void* const* grads, const int64_t* n, const int32_t
 int prfl_grads_sumsq(const void* const* grads, const int64_t* n, const int32_t* type, int64_t count,
                      double* part, int64_t parts, double* sumsq, void* stream);
 /* g *= min(1, max_norm / (norm + eps)), norm = sqrt(sumsq[0]), or with sumsq == NULL the norm of
- * these tensors (part / parts as above); norm[0] (fp32, may be NULL) gets it.  out == NULL (out_type
+ * these tensors (part / parts as above); norm[0] (fp32, may be NULL) gets it, infinity where it is past fp32
+ * (the factor is then formed in 64 bits).  out == NULL (out_type
  * -1): in place (nothing is touched when the factor is 1), else out[i] (out_type, as many elements) =
  * the clipped gradient.  A NaN norm makes every gradient NaN. */
 int prfl_grads_clip(const void* const* grads, void* const* out, const int64_t* n,
