@@ -17,6 +17,7 @@
 #include "common.h"
 
 namespace {
+typedef __attribute__((ext_vector_type(8), aligned(16))) float f32x8;   // two 16-B loads
 constexpr int NT = 256;
 constexpr int MAXV = 5;  // float4 chunks per thread -> C <= 5120 (Wan 14B width)
 
@@ -477,7 +478,8 @@ __global__ __launch_bounds__(NT) void rms_rope_bwd_wave_kernel(
 // RC_ROWS rows RC_R at a time (2 x 16-B loads per thread per row, RC_R rows in flight), the rows'
 // sums of squares reduced across the workgroup through LDS with one barrier per RC_R rows
 // (double-buffered partial array).  The backward keeps its 16 d w partial sums in registers across
-// the block of rows and holds each row's dout / x between its two passes.  Same per-element
+// the block of rows and holds each row's x and, in bf16 as it is defined, the rotated and weighted gradient between its
+// two passes (73920 x 5120: 598 us; 730 with dout held and rotated twice).  Same per-element
 // arithmetic as the kernels above; the sum of squares of a row is added in another order.
 #ifndef RMS_COLS
 #define RMS_COLS 2          // bit 0: forward, bit 1: backward (profiles/r06_ab_norms_cols.txt: the
@@ -653,9 +655,10 @@ __global__ __launch_bounds__(RC_MAXT) void rms_rope_bwd_cols_kernel(
           for (int r = 0; r < 8; ++r) {
             const int e = 8 * h + r;
             const float xhat = bf2f(xv[j][h][r]) * rstd;
-            const float d = bfr(g8[r] * wr[e]);
+            const bf16 d = f2bf(g8[r] * wr[e]);
             p0[e] += g8[r] * bfr(xhat);
-            sp[j] += d * xhat;
+            sp[j] += bf2f(d) * xhat;
+            gv[j][h][r] = d;                 // all that the second pass needs of dout
           }
         }
       }
@@ -674,23 +677,13 @@ __global__ __launch_bounds__(RC_MAXT) void rms_rope_bwd_cols_kernel(
       for (int k = 0; k < nw; ++k) tot += red[buf][j][k];
       const float m = tot / C;
       const float rstd = rstd_in[row];
-      int pf, ph, pw;
-      bool rot;
-      rope_pos(row0 + row, F, Hg, Wg, pf, ph, pw, rot);
-      rot = rot && tab != nullptr;
-      float2 cs[4];
-      if (rot) rope_cs4(tab, pair0, pf, ph, pw, cs);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float g8[8];
-        rot8(gv[j][h], rot, cs, g8);
         bf16x8 o;
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          const int e = 8 * h + r;
           const float xhat = bf2f(xv[j][h][r]) * rstd;
-          const float d = bfr(g8[r] * wr[e]);
-          o[r] = f2bf(rstd * (d - xhat * m));
+          o[r] = f2bf(rstd * (bf2f(gv[j][h][r]) - xhat * m));
         }
         *(bf16x8*)(dx + row * lddx + (h ? c1 : c0)) = o;
       }
@@ -714,13 +707,18 @@ __global__ __launch_bounds__(RC_MAXT) void rms_rope_bwd_cols_kernel(
 #endif
 // (the next row prefetched into a second register set, as RMS_WAVE_PF 2: 0.448 vs 0.449 ms at
 // 720p, profiles/r06_ab_rms_prefetch.txt -- not kept)
+// NV chunks a lane: 20, or 8 for C <= 2048, whose few registers leave room for seven waves a SIMD; FULL (C = 5120):
+// no chunk ends past the row.  All loads of a row come before its sums: 73920 x 5120 fp32 442 us = 5.1 TB/s, bf16 298 us =
+// 5.1 TB/s (482 and 418 us with each chunk added as it is loaded); 20000 x 1536 bf16 24 us (38).  d * d is rounded
+// before it is added, so that the sum's bits do not hang on which products the compiler fuses.
 constexpr int RPW = LN_RPW;   // rows per wave -> 16 rows per workgroup
-__global__ __launch_bounds__(NT) void ln_mod_fwd_lds_kernel(
-    const void* __restrict__ x, int x_bf16, int64_t ldx, int L, int C,
+template <bool XB, int NV, bool FULL>
+__global__ __launch_bounds__(NT, FULL || NV < WV ? 4 : 3) void ln_mod_fwd_lds_kernel(
+    const void* __restrict__ x, int64_t ldx, int L, int C,
     const float* __restrict__ scale, const float* __restrict__ shift, const float* __restrict__ w,
     const float* __restrict__ b, float eps, bf16* __restrict__ out, int64_t ldo,
     float* __restrict__ mean_out, float* __restrict__ rstd_out) {
-  __shared__ f32x4 cA[WV * 64], cB[WV * 64];
+  __shared__ f32x4 cA[NV * 64], cB[NV * 64];
   const int nc = C / 4;
   for (int c = threadIdx.x; c < nc; c += NT) {
     if (w) {
@@ -734,45 +732,42 @@ __global__ __launch_bounds__(NT) void ln_mod_fwd_lds_kernel(
   }
   __syncthreads();
   const int lane = threadIdx.x & 63;
-  const int64_t row0 = ((int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6)) * RPW;
+  const int64_t row0 = ((int64_t)blockIdx.x * (NT / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * RPW;
   for (int rr = 0; rr < RPW; ++rr) {
     const int64_t row = row0 + rr;
     if (row >= L) return;
-    f32x4 v[WV];
+    f32x4 v[NV];
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      v[j] = (f32x4){0, 0, 0, 0};
+      if (FULL || lane + j * 64 < nc) v[j] = ld4(x, row * ldx + (lane + j * 64) * 4, XB);
+    }
     float s = 0.f;
 #pragma unroll
-    for (int j = 0; j < WV; ++j) {
-      const int c = lane + j * 64;
-      if (c < nc) {
-        v[j] = ld4(x, row * ldx + c * 4, x_bf16);
-        s += v[j][0] + v[j][1] + v[j][2] + v[j][3];
-      }
-    }
+    for (int j = 0; j < NV; ++j) s += v[j][0] + v[j][1] + v[j][2] + v[j][3];
     const float mean = wave_sum(s) / C;
     float ss = 0.f;
 #pragma unroll
-    for (int j = 0; j < WV; ++j) {
-      const int c = lane + j * 64;
-      if (c < nc) {
+    for (int j = 0; j < NV; ++j) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float d = v[j][r] - mean;
-          ss += d * d;
-        }
+      for (int r = 0; r < 4; ++r) {
+        const float d = FULL || lane + j * 64 < nc ? v[j][r] - mean : 0.f;
+        ss += mul_rn(d, d);
       }
     }
     const float var = wave_sum(ss) / C;
     const float rstd = rsqrtf(var + eps);
+    asm volatile("" ::: "memory");      // the coefficients are read for each row, not held in 160 registers
 #pragma unroll
-    for (int j = 0; j < WV; ++j) {
+    for (int j = 0; j < NV; ++j) {
       const int c = lane + j * 64;
-      if (c < nc) {
+      if (FULL || c < nc) {
         const f32x4 a = cA[c], bb = cB[c];
         bf16x4 o;
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float xh = (v[j][r] - mean) * rstd;
-          if (!w && x_bf16) xh = bfr(xh);  // WanLayerNorm.type_as(x) for a bf16 input
+          if (!w && XB) xh = bfr(xh);  // WanLayerNorm.type_as(x) for a bf16 input
           o[r] = f2bf(mul_rn(xh, a[r]) + bb[r]);
         }
         *(bf16x4*)(out + row * ldo + c * 4) = o;
@@ -793,9 +788,12 @@ __global__ __launch_bounds__(NT) void ln_mod_fwd_lds_kernel(
 // backward's two column sums (d scale | d w, d shift | d b) stay in registers over the block and
 // its two row sums share one reduction.  Same per-element arithmetic as ln_mod_fwd_lds_kernel /
 // ln_mod_bwd_kernel; the row sums add in another order.
+// The backward holds x and dy of its rows between the two passes: 73920 x 5120 fp32 x 846 us, bf16 x
+// 680 us (951 and 979 with x read again from L2 in the second pass; four waves a SIMD instead of three for fp32 x, with
+// spills, 828, but 391 instead of 364 at 32760 rows).
 #ifndef LN_COLS
-#define LN_COLS 2           // bit 0: forward, bit 1: backward (forward 0.51 ms vs 0.46-0.49 ms for
-#endif                      // ln_mod_fwd_lds_kernel; backward 1.13-1.15 ms either way)
+#define LN_COLS 2           // bit 0: forward, bit 1: backward (forward 0.51 ms, ln_mod_fwd_lds_kernel 0.44)
+#endif
 constexpr int LC_R = 4;             // rows in flight (forward)
 constexpr int LC_RB = 2;            // rows in flight (backward)
 
@@ -916,8 +914,9 @@ __global__ __launch_bounds__(RC_MAXT) void ln_mod_fwd_cols_kernel(
   }
 }
 
+template <bool XB>
 __global__ __launch_bounds__(RC_MAXT) void ln_mod_bwd_cols_kernel(
-    const bf16* __restrict__ dy, int64_t lddy, const void* __restrict__ x, int x_bf16, int64_t ldx,
+    const bf16* __restrict__ dy, int64_t lddy, const void* __restrict__ x, int64_t ldx,
     const float* __restrict__ mean_in, const float* __restrict__ rstd_in, int L, int C,
     const float* __restrict__ scale, const float* __restrict__ w, float* __restrict__ dx,
     int64_t lddx, int dx_accumulate, float* __restrict__ part0, float* __restrict__ part1) {
@@ -942,8 +941,21 @@ __global__ __launch_bounds__(RC_MAXT) void ln_mod_bwd_cols_kernel(
   const int64_t rb = (int64_t)blockIdx.x * RC_ROWS;
   for (int it = 0; it < RC_ROWS / LC_RB; ++it) {
     const int buf = it & 1;
-    bf16x8 dv[LC_RB][2];                  // (x is re-read in the second pass: L1 / L2)
+    bf16x8 dv[LC_RB][2];                  // the rows held between the two passes
+    typename std::conditional<XB, bf16x8, f32x8>::type xv[LC_RB][2];
     float s1[LC_RB], s2[LC_RB];
+#pragma unroll
+    for (int j = 0; j < LC_RB; ++j) {
+      const int64_t row = rb + it * LC_RB + j;
+      if (act && row < L) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          dv[j][h] = *(const bf16x8*)(dy + row * lddy + (h ? c1 : c0));
+          if constexpr (XB) xv[j][h] = *(const bf16x8*)((const bf16*)x + row * ldx + (h ? c1 : c0));
+          else xv[j][h] = *(const f32x8*)((const float*)x + row * ldx + (h ? c1 : c0));
+        }
+      }
+    }
 #pragma unroll
     for (int j = 0; j < LC_RB; ++j) {
       const int64_t row = rb + it * LC_RB + j;
@@ -951,23 +963,19 @@ __global__ __launch_bounds__(RC_MAXT) void ln_mod_bwd_cols_kernel(
       if (act && row < L) {
         const float mean = mean_in[row], rstd = rstd_in[row];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float q8[8];
-          ld_cols(x, row * ldx + (h ? c1 : c0), x_bf16, q8);
-          dv[j][h] = *(const bf16x8*)(dy + row * lddy + (h ? c1 : c0));
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
             const int e = 8 * h + r;
-            const float xhat = (q8[r] - mean) * rstd;
+            const float xhat = ((float)xv[j][h][r] - mean) * rstd;
             const float d = bf2f(dv[j][h][r]);
-            const float xu = (!w && x_bf16) ? bfr(xhat) : xhat;
+            const float xu = (!w && XB) ? bfr(xhat) : xhat;
             p0[e] += d * xu;
             p1[e] += d;
             const float gg = d * m[e];
             s1[j] += gg;
             s2[j] += gg * xhat;
           }
-        }
       }
     }
 #pragma unroll
@@ -993,13 +1001,11 @@ __global__ __launch_bounds__(RC_MAXT) void ln_mod_bwd_cols_kernel(
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float* dp = dx + row * lddx + (h ? c1 : c0);
-        float q8[8];
-        ld_cols(x, row * ldx + (h ? c1 : c0), x_bf16, q8);
         f32x4 o[2];
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
           const int e = 8 * h + r;
-          const float xhat = (q8[r] - mean) * rstd;
+          const float xhat = ((float)xv[j][h][r] - mean) * rstd;
           const float gg = bf2f(dv[j][h][r]) * m[e];
           o[r >> 2][r & 3] = rstd * (gg - m1 - xhat * m2);
         }
@@ -1055,9 +1061,14 @@ extern "C" int prfl_ln_mod_fwd(const void* x, int x_bf16, int64_t ldx, int64_t L
                        dim3(((C / 16) + 63) / 64 * 64), 0, s, x, x_bf16, ldx, (int)L, (int)C, scale,
                        shift, w, b, eps, (bf16*)out, ldo, mean, rstd);
   } else {
-    hipLaunchKernelGGL(ln_mod_fwd_lds_kernel, dim3((L + NT / 64 * RPW - 1) / (NT / 64 * RPW)),
-                       dim3(NT), 0, s, x, x_bf16, ldx, (int)L, (int)C, scale, shift, w, b, eps,
-                       (bf16*)out, ldo, mean, rstd);
+    auto pick = [&](auto xb) {
+      return C == WV * 256 ? ln_mod_fwd_lds_kernel<xb(), WV, true>
+             : C > 2048    ? ln_mod_fwd_lds_kernel<xb(), WV, false>
+                           : ln_mod_fwd_lds_kernel<xb(), 8, false>;
+    };
+    auto kernel = x_bf16 ? pick(std::true_type()) : pick(std::false_type());
+    hipLaunchKernelGGL(kernel, dim3((L + NT / 64 * RPW - 1) / (NT / 64 * RPW)), dim3(NT), 0, s, x, ldx,
+                       (int)L, (int)C, scale, shift, w, b, eps, (bf16*)out, ldo, mean, rstd);
   }
   prfl_prof::set_work((double)L * C * ((x_bf16 ? 2 : 4) + 2));
   prfl_prof::end(KID_LN, s);
@@ -1075,9 +1086,10 @@ extern "C" int prfl_ln_mod_bwd(const void* dy, int64_t lddy, const void* x, int 
   hipStream_t s = (hipStream_t)stream;
   prfl_prof::begin(KID_LN, s);
   if ((LN_COLS & 2) && cols_ok(x, ldx * (x_bf16 ? 1 : 2), dy, lddy, C) && cols_ok(dx, lddx * 2, dx, lddx * 2, C)) {
-    hipLaunchKernelGGL(ln_mod_bwd_cols_kernel, dim3((L + RC_ROWS - 1) / RC_ROWS),
-                       dim3(((C / 16) + 63) / 64 * 64), 0, s, (const bf16*)dy, lddy, x, x_bf16, ldx,
-                       mean, rstd, (int)L, (int)C, scale, w, dx, lddx, dx_accumulate, part0, part1);
+    auto kernel = x_bf16 ? ln_mod_bwd_cols_kernel<true> : ln_mod_bwd_cols_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3((L + RC_ROWS - 1) / RC_ROWS),
+                       dim3(((C / 16) + 63) / 64 * 64), 0, s, (const bf16*)dy, lddy, x, ldx, mean,
+                       rstd, (int)L, (int)C, scale, w, dx, lddx, dx_accumulate, part0, part1);
   } else {
     hipLaunchKernelGGL(ln_mod_bwd_kernel<BWD_ROWS>, dim3((L + BWD_ROWS - 1) / BWD_ROWS), dim3(NT),
                        0, s, (const bf16*)dy, lddy, x, x_bf16, ldx, mean, rstd, (int)L, (int)C, scale,
