@@ -442,13 +442,18 @@ def _rows(t, C):
     return t if t.stride(1) == 1 or C == 1 else t.contiguous()
 
 
+def _last_axis(shape):
+    C = shape[-1] if shape else 0
+    if not 1 <= C <= 16384:
+        raise ValueError(f"layer_norm: a last axis of 1 to 16384, got {tuple(shape)}")
+    return C
+
+
 def layer_norm_fwd(x, w=None, b=None, eps=1e-5, out_dtype=None):
     """LN over the last axis of x [..., C] (C <= 16384), times w plus b ([C] each, or None):
     returns (y in out_dtype or x's, mean, rstd fp32 of x's leading shape)."""
     shape = x.shape
-    C = shape[-1] if shape else 0
-    if not 1 <= C <= 16384:
-        raise ValueError(f"layer_norm: a last axis of 1 to 16384, got {tuple(shape)}")
+    C = _last_axis(shape)
     dev = _one_device("layer_norm", x, w, b)
     ydt = x.dtype if out_dtype is None else out_dtype
     xt, yt, wt, pw, pb = _type(x.dtype, "layer_norm x"), _type(ydt, "layer_norm out_dtype"), 0, None, None
@@ -483,7 +488,7 @@ def _addr(t):
 def layer_norm_bwd(dy, x, mean, rstd, w=None, want_dx=True, want_dw=None, want_db=True):
     """Backward of layer_norm_fwd: (dx in x's type, dw, db fp32 [C]; None where not wanted).  dy has
     the forward's output type; dw is given by default where w is."""
-    C = x.shape[-1]
+    C = _last_axis(x.shape)
     dev = _one_device("layer_norm", x, dy, mean, rstd, w)
     if dy.shape != x.shape or mean.numel() * C != x.numel() or rstd.numel() != mean.numel():
         raise ValueError("layer_norm: dy has x's shape, mean and rstd one value a row")
@@ -612,6 +617,9 @@ def clip_grads(grads, max_norm, eps=1e-6, out=None, sumsq=None):
 
 
 # ------------------------------------------------------------ microscaled fp4 (csrc/mxfp4.hip) --
+MX_MOST = 1 << 24              # columns of a tiled matrix, and rows of one that is multiplied by
+
+
 def _mx_shape(rows, cols):
     return -(-rows // 64), -(-cols // 128)
 
@@ -619,8 +627,8 @@ def _mx_shape(rows, cols):
 def quant_mxfp4(x):
     """x [M, K] (fp32 / bf16 / fp16, row-strided) -> (q uint8 [M/64, K/128, 4, 64, 16], s uint8
     [M/64, K/128, 64, 4]): e2m1 codes and e8m0 scales in the tiled layout of include/prfl_hip.h."""
-    if x.dim() != 2 or x.shape[1] < 1:
-        raise ValueError(f"quant_mxfp4: [M, K] with K >= 1, got {tuple(x.shape)}")
+    if x.dim() != 2 or not 1 <= x.shape[1] <= MX_MOST:
+        raise ValueError(f"quant_mxfp4: [M, K] with K of 1 to 2^24, got {tuple(x.shape)}")
     dev = _one_device("quant_mxfp4", x)
     xt = _type(x.dtype, "quant_mxfp4")
     M, K = x.shape
@@ -634,7 +642,7 @@ def quant_mxfp4(x):
 
 
 def _mx_check(what, q, s, rows, cols):
-    if cols < 1 or rows < 0:
+    if not 1 <= cols <= MX_MOST or rows < 0:
         raise ValueError(f"{what}: a [{rows}, {cols}] matrix")
     G, S = _mx_shape(rows, cols)
     if (q.shape != (G, S, 4, 64, 16) or s.shape != (G, S, 64, 4) or q.dtype != torch.uint8
@@ -659,7 +667,7 @@ def dequant_mxfp4(q, s, rows, cols, out_dtype=BF16):
 def linear_mxfp4(x, wq, ws, out_features, bias=None):
     """y [..., N] bf16 = x W^T + bias on the block-scaled MFMA: x [..., K] (fp32 / bf16 / fp16) is
     quantised to microscaled fp4 in the call, (wq, ws) = quant_mxfp4(W [N, K]), bias bf16 [N]."""
-    if x.dim() < 1 or x.shape[-1] < 1 or out_features < 1:
+    if x.dim() < 1 or x.shape[-1] < 1 or not 1 <= out_features <= MX_MOST:
         raise ValueError(f"linear_mxfp4: x is [..., K], got {tuple(x.shape)} to {out_features}")
     K, N = x.shape[-1], out_features
     dev = _one_device("linear_mxfp4", x, wq, ws, bias)
@@ -681,6 +689,8 @@ def linear_mxfp4_dx(dy, wq, ws, in_features):
     """dx [..., K] bf16 = dy W of linear_mxfp4, x's quantisation taken as the identity: W is read
     back to bf16 (exact) and multiplied on the bf16 MFMA, for small products in one launch.  dy [..., N] is
     taken in bf16."""
+    if dy.dim() < 1 or not 1 <= dy.shape[-1] <= MX_MOST:
+        raise ValueError(f"linear_mxfp4_dx: dy is [..., N], got {tuple(dy.shape)}")
     N, K = dy.shape[-1], in_features
     dev = _one_device("linear_mxfp4_dx", dy, wq, ws)
     _mx_check("linear_mxfp4_dx", wq, ws, N, K)

@@ -105,6 +105,25 @@ def test_mxfp4_refusals(ops):
         refuses(lambda: ops.linear_mxfp4_dx(E(3, 100, t=F64), q, s, 100))
 
 
+def test_shapes_that_only_one_direction_refused(ops):
+    with FakeTensorMode():
+        E = lambda *s, t=F32: torch.empty(s, device="cuda", dtype=t)  # noqa: E731
+        U = lambda *s: E(*s, t=torch.uint8)  # noqa: E731
+        refuses(lambda: ops.layer_norm_bwd(E(), E(), E(), E()))
+        refuses(lambda: ops.layer_norm_bwd(E(4, 0), E(4, 0), E(4), E(4)))
+        refuses(lambda: ops.layer_norm_bwd(E(4, 16385), E(4, 16385), E(4), E(4)))
+        q, s = U(2, 1, 4, 64, 16), U(2, 1, 64, 4)
+        refuses(lambda: ops.linear_mxfp4_dx(E(), q, s, 100))
+        refuses(lambda: ops.linear_mxfp4_dx(E(3, 0, t=BF16), q[:0], s[:0], 100))
+        wide = (1 << 24) + 1
+        refuses(lambda: ops.quant_mxfp4(E(1, wide)))
+        refuses(lambda: ops.dequant_mxfp4(U(1, 131073, 4, 64, 16), U(1, 131073, 64, 4), 1, wide))
+        refuses(lambda: ops.linear_mxfp4(E(1, wide), U(1, 131073, 4, 64, 16), U(1, 131073, 64, 4), 1))
+        refuses(lambda: ops.linear_mxfp4(E(1, 8), U(262145, 1, 4, 64, 16), U(262145, 1, 64, 4), wide))
+        refuses(lambda: ops.linear_mxfp4_dx(E(1, wide), U(262145, 1, 4, 64, 16), U(262145, 1, 64, 4), 8))
+        refuses(lambda: ops.linear_mxfp4_dx(E(1, 8), U(1, 131073, 4, 64, 16), U(1, 131073, 64, 4), wide))
+
+
 def test_clip_refusals(ops):
     refuses(lambda: ops.clip_grads([], 1.0))
     with FakeTensorMode():
