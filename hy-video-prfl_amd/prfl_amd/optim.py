@@ -12,7 +12,9 @@
                       update order (attach(): the last blocks a forward reads) covering f of the
                       parameters and keeps the rest in HBM: the 480p plan (C3), where the whole
                       stream (~4 s of PCIe per update) does not hide under a 480p rollout but a
-                      fifth of it does, and frees 23 GB of HBM.
+                      fifth of it does, and frees 23 GB of HBM.  What the host cannot pin (drivers
+                      limit it; a warning names the amount) is kept in pageable memory: the same
+                      values, but its copies run at 30 / 17 GB/s instead of 57 and hold step() up.
     ``overlap``       the update runs on a side stream and step() returns without making the
                       caller's stream wait.  Every parameter gets a ready event; ``attach(model)``
                       installs forward pre-hooks so the first forward that reads a parameter
@@ -34,11 +36,43 @@
 * ``clip_grads_``     — the same over fp32 / bf16 / fp16 gradients in a launch per 128 tensors, the
                         squares summed in 64 bits and a fixed order (csrc/grads.hip).
 """
+import warnings
 import weakref
 
 import torch
 
 from . import ops
+
+SLAB = 1 << 29          # fp32 elements (2 GiB) of pinned memory per allocation
+
+
+class _HostMemory:
+    """`need` fp32 zeros in pinned host memory, cut from slabs of 2^29 elements (torch's allocator of pinned memory
+    rounds each tensor up to a power of two: 172 GB for the 14B DiT's 114 GB of moments), and in pageable memory once
+    no more can be pinned."""
+
+    def __init__(self, need):
+        self.need, self.slab, self.used, self.full = need, None, 0, False
+
+    def zeros(self, n):
+        """(n zeros, whether they are pinned)"""
+        if not self.full:
+            try:
+                return self._pinned(n).zero_(), True
+            except RuntimeError as e:                   # the driver's limit, whatever its type of error
+                self.full = True
+                warnings.warn(f"AdamW: no more host memory can be pinned ({str(e).splitlines()[0]}): "
+                              f"{4e-9 * self.need:.1f} GB of moments are kept in pageable memory, whose copies are slower")
+        return torch.zeros(n, dtype=torch.float32), False
+
+    def _pinned(self, n):
+        if self.slab is None or self.used + n > self.slab.numel():
+            self.slab = torch.empty(max(n, min(SLAB, self.need)), dtype=torch.float32, pin_memory=True)
+            self.used = 0
+        at = self.used
+        self.used += -(-n // 64) * 64
+        self.need -= -(-n // 64) * 64
+        return self.slab[at:at + n]
 
 
 class AdamW:
@@ -56,6 +90,8 @@ class AdamW:
         self._groups = None         # ZeRO-1 layout (lazy: attach() may still re-order)
         self.lr, self.betas, self.eps, self.weight_decay = lr, betas, eps, weight_decay
         self.state = {}             # param -> (exp_avg, exp_avg_sq) of this rank's range of it
+        self._host = None           # where the moments on the host come from
+        self._pageable = set()      # the parameters whose moments could not be pinned
         self.step_count = 0         # optimizer steps taken
         self._pstep = {}            # per-parameter update count (torch's state['step']): the bias
         #                             correction of a parameter that skipped a window lags behind
@@ -157,8 +193,13 @@ class AdamW:
             self._layout()
             a, b = self._range[p]
             if p in self._host_params():
-                st = (torch.zeros(b - a, dtype=torch.float32, pin_memory=True),
-                      torch.zeros(b - a, dtype=torch.float32, pin_memory=True))
+                if self._host is None:
+                    mine = [self._range[q] for q in self._host_params() if q in self._range]
+                    self._host = _HostMemory(sum(2 * (-(-(d - c) // 64) * 64) for c, d in mine))
+                (m, pinned), (v, also) = self._host.zeros(b - a), self._host.zeros(b - a)
+                st = (m, v)
+                if not (pinned and also):
+                    self._pageable.add(p)
             else:
                 st = (torch.zeros(b - a, dtype=torch.float32, device=p.device),
                       torch.zeros(b - a, dtype=torch.float32, device=p.device))
@@ -209,7 +250,7 @@ class AdamW:
             raise RuntimeError("attach() must precede the first step: the update order decides "
                                "the host-moment tail and the ZeRO-1 shards")
         reinit = bool(self.state)           # zero moments from init_state(): re-placed below
-        self.state = {}
+        self.state, self._host, self._pageable = {}, None, set()
         self._host_set = None
         mine = {id(p) for p in self.params}
         lists = [[p for p in rest if id(p) in mine]] + \
@@ -379,8 +420,9 @@ class AdamW:
             with torch.cuda.stream(cp):
                 if i >= k:
                     cp.wait_event(d2h_ev[i - k])
-                m_d[:n].copy_(m_h, non_blocking=True)
-                v_d[:n].copy_(v_h, non_blocking=True)
+                free = p not in self._pageable      # (a copy of pageable memory is waited for)
+                m_d[:n].copy_(m_h, non_blocking=free)
+                v_d[:n].copy_(v_h, non_blocking=free)
                 h2d_ev[i] = torch.cuda.Event()
                 h2d_ev[i].record(cp)
 
@@ -402,8 +444,8 @@ class AdamW:
             m_h, v_h = self._state(p)
             with torch.cuda.stream(dn):
                 dn.wait_event(ev)
-                m_h.copy_(m_d[:n], non_blocking=True)
-                v_h.copy_(v_d[:n], non_blocking=True)
+                m_h.copy_(m_d[:n], non_blocking=p not in self._pageable)
+                v_h.copy_(v_d[:n], non_blocking=p not in self._pageable)
                 d2h_ev[i] = torch.cuda.Event()
                 d2h_ev[i].record(dn)
             if i + k < len(units):
