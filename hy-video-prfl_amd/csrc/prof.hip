@@ -4,6 +4,10 @@
 // Clock slots: while on, a kernel that takes one (the self-attention forward) has its workgroup
 // 0 write (shader cycles, 100 MHz ticks) elapsed over its lifetime (s_memtime / s_memrealtime):
 // the effective shader clock during the launches the roofline is computed from.
+//
+// Launches may come from two threads at once (the optimizer's, autograd's): the records are kept under a lock, and what
+// belongs to the launch under way is the thread's own.
+#include <mutex>
 #include <vector>
 
 #include "common.h"
@@ -15,10 +19,11 @@ struct Rec {
   double work;
 };
 bool g_on = false;
+std::mutex g_lock;                 // over g_recs, g_pool and g_clk_n
 std::vector<Rec> g_recs;
 std::vector<hipEvent_t> g_pool;
-int g_open[KID_COUNT + 8];
-double g_pending_work = 0.0;
+thread_local int t_open[KID_COUNT + 8];
+thread_local double t_pending_work = 0.0;
 constexpr int CLK_CAP = 1 << 15;   // launches per window
 unsigned long long* g_clk = nullptr;
 int g_clk_n = 0;
@@ -38,23 +43,27 @@ hipEvent_t get_event() {
 namespace prfl_prof {
 void begin(int kid, hipStream_t s) {
   if (!g_on) return;
+  std::lock_guard<std::mutex> hold(g_lock);
   Rec r{kid, get_event(), get_event(), 0.0};
   if (!r.a || !r.b) return;
   (void)hipEventRecord(r.a, s);
-  g_open[kid] = (int)g_recs.size();
+  t_open[kid] = (int)g_recs.size();
   g_recs.push_back(r);
 }
 void end(int kid, hipStream_t s) {
   if (!g_on) return;
-  if (g_recs.empty()) return;
-  Rec& r = g_recs[g_open[kid]];
-  r.work = g_pending_work;
-  g_pending_work = 0.0;
+  std::lock_guard<std::mutex> hold(g_lock);
+  if (t_open[kid] >= (int)g_recs.size()) return;
+  Rec& r = g_recs[t_open[kid]];
+  r.work = t_pending_work;
+  t_pending_work = 0.0;
   (void)hipEventRecord(r.b, s);
 }
-void set_work(double w) { g_pending_work = w; }
+void set_work(double w) { t_pending_work = w; }
 unsigned long long* clk_slot() {
-  if (!g_on || !g_clk || g_clk_n >= CLK_CAP) return nullptr;
+  if (!g_on || !g_clk) return nullptr;
+  std::lock_guard<std::mutex> hold(g_lock);
+  if (g_clk_n >= CLK_CAP) return nullptr;
   return g_clk + 2 * (g_clk_n++);
 }
 }  // namespace prfl_prof
@@ -113,6 +122,7 @@ extern "C" int prfl_prof_collect(int64_t* counts, double* ms, double* work, int 
     ms[k] = 0.0;
     work[k] = 0.0;
   }
+  std::lock_guard<std::mutex> hold(g_lock);
   for (auto& r : g_recs) {
     if (hipEventSynchronize(r.b) != hipSuccess) return -1;
     float t = 0.f;

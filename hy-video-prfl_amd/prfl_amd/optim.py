@@ -14,7 +14,9 @@
                       stream (~4 s of PCIe per update) does not hide under a 480p rollout but a
                       fifth of it does, and frees 23 GB of HBM.  What the host cannot pin (drivers
                       limit it; a warning names the amount) is kept in pageable memory: the same
-                      values, but its copies run at 30 / 17 GB/s instead of 57 and hold step() up.
+                      values, but its copies run at 30 / 17 GB/s instead of 57, each waited for by
+                      the host: in step(), or with ``overlap`` in a thread of its own, behind the
+                      pinned ones and beside the next forward.
     ``overlap``       the update runs on a side stream and step() returns without making the
                       caller's stream wait.  Every parameter gets a ready event; ``attach(model)``
                       installs forward pre-hooks so the first forward that reads a parameter
@@ -36,6 +38,7 @@
 * ``clip_grads_``     — the same over fp32 / bf16 / fp16 gradients in a launch per 128 tensors, the
                         squares summed in 64 bits and a fixed order (csrc/grads.hip).
 """
+import concurrent.futures
 import warnings
 import weakref
 
@@ -92,6 +95,8 @@ class AdamW:
         self.state = {}             # param -> (exp_avg, exp_avg_sq) of this rank's range of it
         self._host = None           # where the moments on the host come from
         self._pageable = set()      # the parameters whose moments could not be pinned
+        self._thread = None         # issues their updates where step() does not wait for them
+        self._tail = None           # its work under way
         self.step_count = 0         # optimizer steps taken
         self._pstep = {}            # per-parameter update count (torch's state['step']): the bias
         #                             correction of a parameter that skipped a window lags behind
@@ -224,11 +229,21 @@ class AdamW:
             return
         cur = torch.cuda.current_stream(ps[0].device)
         for p in ps:
-            cur.wait_event(self._ready.pop(p))
+            ready = self._ready.pop(p)
+            if isinstance(ready, concurrent.futures.Future):      # not issued yet, perhaps
+                ready = ready.result()
+            cur.wait_event(ready)
+
+    def _join(self):
+        """The thread's work issued (it uses the ring, the streams and the step counts of its step)."""
+        if self._tail is not None:
+            tail, self._tail = self._tail, None
+            tail.result()
 
     def synchronize(self):
         """All updates visible to the current stream and the host moments complete."""
         self.wait()
+        self._join()
         if self._streams is not None:
             for s in self._streams:
                 s.synchronize()
@@ -282,6 +297,7 @@ class AdamW:
             # only the forward pre-hooks of attach() order that write after the zeroing.  Checked
             # before any counter moves, so a caller may attach() and call step() again.
             raise RuntimeError("AdamW(overlap=True).step(zero_grad=True) needs attach(model) first")
+        self._join()
         self.step_count += 1
         lr = self.param_groups[0]["lr"]
         for p in live:
@@ -331,9 +347,14 @@ class AdamW:
                             g[b:].zero_()
                 # device-resident moments first, then the streamed ones: their first H2D copies
                 # start on `cp` at once, beside the device updates
+                later = self._pageable if self.overlap and not self.shard else ()
                 done = self._update_device([u for u in units if u[0] not in host], lr, zero_grad)
-                done.update(self._update_streamed([u for u in units if u[0] in host], lr, opt, cp,
-                                                  dn if self.duplex else cp, zero_grad))
+                done.update(self._update_streamed(
+                    [u for u in units if u[0] in host and u[0] not in later], lr, opt, cp,
+                    dn if self.duplex else cp, zero_grad))
+                paged = [u for u in units if u[0] in later]
+                if paged:
+                    done.update(self._update_in_thread(paged, lr, opt, cp, dn if self.duplex else cp, zero_grad))
                 if self.shard:
                     for p in glive:
                         if p in done:
@@ -388,7 +409,34 @@ class AdamW:
             done[p] = ev
         return done
 
-    def _update_streamed(self, units, lr, opt, cp, dn, zero_grad=False):
+    def _update_in_thread(self, units, lr, opt, cp, dn, zero_grad):
+        """_update_streamed from a thread: {p: Future of its ready event}.  The gradients are taken now, so
+        that the caller may drop or replace them."""
+        grads = {}
+        for p, _, _ in units:
+            g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
+            if zero_grad and g is not p.grad:
+                p.grad.zero_()
+            grads[p] = g
+        ready = {p: concurrent.futures.Future() for p, _, _ in units}
+
+        def run():
+            try:
+                torch.cuda.set_device(units[0][0].device)
+                with torch.no_grad(), torch.cuda.stream(opt):
+                    self._update_streamed(units, lr, opt, cp, dn, zero_grad, grads, ready)
+            except BaseException as e:
+                for f in ready.values():
+                    if not f.done():
+                        f.set_exception(e)
+                raise
+
+        if self._thread is None:
+            self._thread = concurrent.futures.ThreadPoolExecutor(1, "AdamW")
+        self._tail = self._thread.submit(run)
+        return ready
+
+    def _update_streamed(self, units, lr, opt, cp, dn, zero_grad=False, grads=None, ready=None):
         """Moments host -> ring -> kernel -> host with the two directions on two copy streams, so
         PCIe carries both at once (full duplex): `cp` H2D(0..k-1), then H2D(i+k) into the slot
         once D2H(i) on `dn` has drained it; `dn` D2H(i) after kernel(i) on `opt`.  (One stream for
@@ -432,15 +480,17 @@ class AdamW:
             n = b - a
             m_d, v_d = slots[i % k]
             opt.wait_event(h2d_ev[i])
-            g = p.grad if p.grad.is_contiguous() else p.grad.contiguous()
+            g = grads[p] if grads else p.grad if p.grad.is_contiguous() else p.grad.contiguous()
             ops.adamw_(self._flat(p.data, a, b), self._flat(g, a, b), m_d[:n], v_d[:n], lr,
                        self.betas[0], self.betas[1], self.eps, self.weight_decay, self._pstep[p],
                        zero_grad=zero_grad)
-            if zero_grad and g is not p.grad:
+            if not grads and zero_grad and g is not p.grad:
                 p.grad.zero_()
             ev = torch.cuda.Event()
             ev.record(opt)
             done[p] = ev
+            if ready:
+                ready[p].set_result(ev)
             m_h, v_h = self._state(p)
             with torch.cuda.stream(dn):
                 dn.wait_event(ev)

@@ -73,3 +73,79 @@ def test_slabs_waste_nothing_of_note():
     need = sum(2 * (-(-p.numel() // 64) * 64) for p in params)
     assert {m.untyped_storage().nbytes() for pair in opt.state.values() for m in pair} == {4 * need}
     assert opt._host.need == 0 and all(m.is_pinned() and not m.any() for pair in opt.state.values() for m in pair)
+
+
+class Toy(torch.nn.Module):
+    def __init__(self):
+        super().__init__()
+        self.emb = torch.nn.Linear(16, 640)
+        self.blocks = torch.nn.ModuleList([torch.nn.Linear(640, 640) for _ in range(5)])
+        self.head = torch.nn.Linear(640, 3)
+
+    def forward(self, x):
+        x = self.emb(x)
+        for b in self.blocks:
+            x = torch.tanh(b(x))
+        return self.head(x)
+
+
+@pytest.mark.parametrize("limit", (0, 2_000_000))
+@pytest.mark.parametrize("keep", (False, True))
+def test_forward_behind_an_update_from_the_thread(monkeypatch, limit, keep):
+    """forwards wait block by block for updates that are still to be issued; gradients may be dropped or are zeroed"""
+    from prfl_amd import optim
+    torch.manual_seed(0)
+    ma = Toy().to(DEV)
+    mb = Toy().to(DEV)
+    mb.load_state_dict(ma.state_dict())
+    x = torch.randn(32, 16, device=DEV)
+    oa = optim.AdamW(list(ma.parameters()), lr=1e-2)
+    monkeypatch.setattr(optim, "SLAB", 1 << 19)
+    limit_pinning(monkeypatch, limit)
+    ob = optim.AdamW(list(mb.parameters()), lr=1e-2, state_on_host=True, overlap=True, ring_slots=2)
+    ob.attach(mb)
+    with pytest.warns(UserWarning, match="pageable"):
+        ob.init_state()
+    assert ob._pageable and (limit == 0 or len(ob._pageable) < len(ob.params))
+    for k in range(5):
+        la, lb = ma(x).square().mean(), mb(x).square().mean()
+        assert torch.equal(la, lb), k
+        la.backward()
+        lb.backward()
+        if k == 2:                                       # a gradient that does not lie in order
+            g = mb.blocks[3].weight.grad
+            mb.blocks[3].weight.grad = g.t().contiguous().t()
+        oa.step()
+        ob.step(zero_grad=keep)
+        oa.zero_grad()
+        if not keep:
+            ob.zero_grad()
+        elif k == 2:
+            ob.wait()
+            assert not any(p.grad.any() for p in mb.parameters())
+            assert not any(ob._fresh(p) for p in mb.parameters())
+    ob.synchronize()
+    for p, q in zip(ma.parameters(), mb.parameters()):
+        assert torch.equal(p, q)
+        for s, t in zip(oa.state[p], ob.state[q]):
+            assert torch.equal(s.flatten().cpu(), t)
+
+
+def test_what_fails_in_the_thread_is_raised_where_it_is_waited_for(monkeypatch):
+    from prfl_amd import optim
+    params = [torch.nn.Parameter(torch.zeros(100, device=DEV)) for _ in range(3)]
+    limit_pinning(monkeypatch, 0)
+    opt = optim.AdamW(params, state_on_host=True, overlap=True)
+    with pytest.warns(UserWarning, match="pageable"):
+        opt.init_state()
+    for p in params:
+        p.grad = torch.ones_like(p)
+
+    def broken(*a, **k):
+        raise ValueError("no update")
+    monkeypatch.setattr(optim.ops, "adamw_", broken)
+    opt.step()
+    with pytest.raises(ValueError, match="no update"):
+        opt.wait()
+    with pytest.raises(ValueError, match="no update"):
+        opt.synchronize()
