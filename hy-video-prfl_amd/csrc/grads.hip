@@ -7,8 +7,9 @@
 // (nothing is copied to the device, and a captured graph holds them by value).  The squares are
 // summed in 64 bits: an fp32 square leaves its range for |g| above 1.8e19 or below 1e-22, and the
 // sum runs over up to 1e10 elements.  Partial sums are written per workgroup and joined in a fixed
-// order, by every workgroup of the clip for itself (at most 16 KB of them; a launch of its own
-// for that would cost a small list a third of its time): no atomics, the same bits every time.
+// order, by every workgroup of the clip for itself (16 KB of them for up to 1024 tensors, 2 KB more for each
+// further 128; a launch of its own for that would cost a small list a third of its time): no atomics, the same
+// bits every time.
 #include <math.h>
 
 #include <algorithm>

@@ -435,10 +435,11 @@ __global__ __launch_bounds__(64 * dx_waves(MT)) void mx_dx_rows_kernel(const T* 
 //
 // WT 4: 32760 x 13824 x 5120 takes 1.10 ms = 4.2 PFLOP/s.  MFMAs alone on random operands run at 6.0 to 6.6 PFLOP/s (the
 // clock falls to 1.5 GHz); here they are busy 57 % of 1.78 GHz.  A tile takes 65 k cycles: first loads 2.9 k, 40 steps
-// of 1316 (1024 of MFMAs), image 3.7 k, stores 4.9 k, the next workgroup 1.3 k.  Power bounds it, not those cycles: measured
-// and dropped, 1.10 ms each, were one workgroup per CU walking its tiles as one stream of steps, the finished tile
-// stored during the next one's, and the 16 x 16 x 128 MFMAs (alone 13 % faster), at 1.90 GHz for more cycles.  With the
-// operands' DMA left out it takes 0.84 ms, with a few KiB of operands from L2 1.08.
+// of 1316 (1024 of MFMAs), image 3.7 k, stores 4.9 k, the next workgroup 1.3 k.  Two things bound it.  The operands' way
+// into LDS: without the DMA it takes 0.84 ms (from a few KiB of L2 instead of HBM still 1.08, so not HBM).  And power,
+// which gives fewer cycles a lower clock: 1.10 ms each, measured and dropped, were one workgroup per CU walking its
+// tiles as one stream of steps, the finished tile stored during the next one's, and the 16 x 16 x 128 MFMAs (alone 13 %
+// faster), at 1.90 GHz for more cycles.
 // WT 2: LDS sets the time, 48 KiB a step per CU against 256 cycles of MFMAs (512 x 5120 x 4096: 12 us, of which 5 us are
 // launch, first loads and stores).  Measured and dropped, no faster: an eight-slot ring, fragments read a whole
 // step ahead, and two groups of waves that share K.
@@ -656,8 +657,10 @@ void launch_product(const MxArgs& a, hipStream_t st) {
   }
 }
 
-// One launch for both: every workgroup quantises all of x, so only while that is a block a thread (5120 x 5120,
-// one row: 5.2 us against 4.3 + 4.3 in two launches).
+// One launch for both: every workgroup quantises all of x, so only while that is a block a thread.  Kernel times in us
+// against two launches (rows x columns of y x K): 1 x 5120 x 5120 4.4 / 7.7, 6 x 5120 x 5120 5.5 / 7.7, 1 x 13824 x 5120
+// 10.8 / 13.4, 1 x 30000 x 4096 18.2 / 17.5.  The columns are not in the rule, though each workgroup of 32 of them
+// quantises x again: 8 x 13824 x 4096 15.0 / 13.3, 8 x 65536 x 4096 55 / 27.
 bool fused(int64_t M, int64_t K) { return M <= 32 && M * ((K + 31) / 32) <= ROWS_FUSED; }
 
 // dx in one launch while its workgroups are few: kernel times in us against W read back to bf16 and multiplied by the
