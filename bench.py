@@ -410,6 +410,7 @@ def main():
         ops.prof_clock()                         # drop clock slots of anything before the window
         if prfl:
             tr.reducer.collect_tail_ms()     # drop the warm-up's records
+            tr.optimizer.synchronize()       # the warm-up's last update, also what a thread still issues
         torch.cuda.synchronize()
         if world > 1:
             dist.barrier()
@@ -420,7 +421,7 @@ def main():
             # main stream only: the reward step's optimizer update (moments streamed over PCIe
             # on the optimizer's side streams) runs on under the next iteration's first forward,
             # each block waiting for its own parameters (optim.py attach), as in a training loop;
-            # the synchronize after the loop puts the last update inside the timed window
+            # the synchronizes after the loop put the last update inside the timed window
             torch.cuda.current_stream().synchronize()
             steps += 1
             t_it = time.time() - t0 - sum(durs)
@@ -432,6 +433,8 @@ def main():
                 dist.all_reduce(go, op=dist.ReduceOp.MIN)
             if go.item() == 0.0:
                 break
+        if prfl:
+            tr.optimizer.synchronize()       # the last update, also what a thread still issues
         torch.cuda.synchronize()
         if world > 1:
             dist.barrier()

@@ -16,7 +16,8 @@
                       limit it; a warning names the amount) is kept in pageable memory: the same
                       values, but its copies run at 30 / 17 GB/s instead of 57, each waited for by
                       the host: in step(), or with ``overlap`` in a thread of its own, behind the
-                      pinned ones and beside the next forward.
+                      pinned ones and beside the next forward (then synchronize() covers them; a
+                      device-wide synchronize does not cover what the thread has yet to issue).
     ``overlap``       the update runs on a side stream and step() returns without making the
                       caller's stream wait.  Every parameter gets a ready event; ``attach(model)``
                       installs forward pre-hooks so the first forward that reads a parameter
