@@ -12,8 +12,8 @@
                       update order (attach(): the last blocks a forward reads) covering f of the
                       parameters and keeps the rest in HBM: the 480p plan (C3), where the whole
                       stream (~4 s of PCIe per update) does not hide under a 480p rollout but a
-                      fifth of it does, and frees 23 GB of HBM.  What the host cannot pin (drivers
-                      limit it; a warning names the amount) is kept in pageable memory: the same
+                      fifth of it does, and frees 23 GB of HBM.  What the host cannot pin (there are
+                      limits; a warning names the amount) is kept in pageable memory: the same
                       values, but its copies run at 30 / 17 GB/s instead of 57, each waited for by
                       the host: in step(), or with ``overlap`` in a thread of its own, behind the
                       pinned ones and beside the next forward (then synchronize() covers them; a
@@ -63,7 +63,7 @@ class _HostMemory:
         if not self.full:
             try:
                 return self._pinned(n).zero_(), True
-            except RuntimeError as e:                   # the driver's limit, whatever its type of error
+            except RuntimeError as e:                   # the limit on pinned memory, as whatever error
                 self.full = True
                 warnings.warn(f"AdamW: no more host memory can be pinned ({str(e).splitlines()[0]}): "
                               f"{4e-9 * self.need:.1f} GB of moments are kept in pageable memory, whose copies are slower")

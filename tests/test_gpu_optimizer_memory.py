@@ -11,7 +11,7 @@ SHAPES = [(3000,), (257, 33), (5,), (1024, 64), (7, 11), (300, 300), (64,)]
 
 
 def limit_pinning(monkeypatch, elements):
-    """the driver pins `elements` fp32 values and then no more"""
+    """as if `elements` fp32 values could be pinned and then no more"""
     from prfl_amd import optim
     empty, left = torch.empty, [elements]
 
